@@ -34,6 +34,9 @@
  *   uaii_hip_gemm_rmsnorm/_add/_swiglu  the same three at M>1 (prefill)
  *   uaii_hip_attention_prefill attention_kv_f32 for a run of prompt positions
  *                              (the reference feeds them one per step)
+ *   uaii_hip_kv_append_batch / KvCache::append_layer and attention_kv_f32 for the caches
+ *   _attention_batch / _prompt of a batch (f32, f16 or 8-bit), with score options that
+ *                              have no counterpart in the reference
  * and the reference ROCm stub's launchers it supersedes
  * (libs/uaii-backends/src/rocm_kernels.hpp:10-14: launch_add_f32, launch_rmsnorm_f32).
  */
@@ -211,6 +214,68 @@ UAII_HIP_API int uaii_hip_attention_prefill(const float* q, const void* kcache,
                                             const void* vcache, int64_t max_seq, int n_heads,
                                             int n_kv_heads, int head_dim, int64_t p0, int64_t m,
                                             float* out, void* stream);
+
+/* ---- caches of a batch --------------------------------------------------------- */
+/* K and V of several sequences, as f32, f16 or 8-bit values. One sequence's K (or V) is
+ * head-major, [n_kv_heads][max_seq][head_dim], the layout of the entry points above; an
+ * UAII_HIP_KV_Q8 cache holds bytes there and, behind them, [n_kv_heads][max_seq] f32
+ * scales: a value is (byte - 128) * scale, a head's row having one scale, max |x| / 127
+ * (the next lower number where 127 of it would pass the end of f32). Rows with an infinity or a NaN read back as NaN. A batch's caches lie one behind the
+ * other, sequence s at s * uaii_hip_kv_cache_bytes. Caches are 16-byte aligned; head_dim
+ * is a multiple of 16 up to 256. */
+#define UAII_HIP_KV_F32 0
+#define UAII_HIP_KV_F16 1
+#define UAII_HIP_KV_Q8 2
+/* Bytes of one sequence's K (or V); -1 for a layout that is not supported. */
+UAII_HIP_API int64_t uaii_hip_kv_cache_bytes(int kv_type, int n_kv_heads, int64_t max_seq, int head_dim);
+/* rows rows of each of n_seq sequences into their caches: row i of sequence s ([n_seq *
+ * rows][ld] floats in k and v, n_kv_heads * head_dim used) goes to position p0 + past[s] + i,
+ * past a device array of n_seq lengths or NULL for none. Rows whose position is outside
+ * the cache are not written; without past such a call returns -1
+ * (KvCache::append_layer, include/uaii/runtime/kv_cache.hpp:80-120, for one sequence). */
+UAII_HIP_API int uaii_hip_kv_append_batch(const float* k, const float* v, int64_t ld, void* kcache, void* vcache,
+                                          int kv_type, int64_t n_seq, int64_t rows, int n_kv_heads, int head_dim,
+                                          int64_t max_seq, int64_t p0, const int32_t* past, void* stream);
+/* The same rows of one cache (K or V) back as floats, out [n_seq * rows][ld]; rows outside
+ * the cache are left as they were. */
+UAII_HIP_API int uaii_hip_kv_read(const void* cache, int kv_type, int64_t n_seq, int64_t rows, int n_kv_heads,
+                                  int head_dim, int64_t max_seq, int64_t p0, const int32_t* past, float* out,
+                                  int64_t ld, void* stream);
+/* How scores come from q . k, and which keys a query at position i sees besides what the
+ * call says. The key at position j has the score
+ *   s = scale * q . k_j, then softcap * tanh(s / softcap), then s - slopes[head] * |i - j|. */
+typedef struct uaii_hip_score_options {
+  uint32_t struct_size;
+  float scale;         /* 0: 1 / sqrt(head_dim) */
+  float softcap;       /* 0: none */
+  const float* slopes; /* device, one for each query head; NULL: none */
+  int64_t window;      /* > 0: keys at i - window + 1 and after only; 0: all */
+} uaii_hip_score_options;
+UAII_HIP_API void uaii_hip_score_options_init(uaii_hip_score_options* options);
+/* Attention of one query for each of n_seq sequences (q, out: [n_seq][ldq], [n_seq][ldo],
+ * n_heads * head_dim used): over a prefix that all share, positions 0 .. n_prefix - 1 of one
+ * sequence's cache of prefix_seq positions (kprefix, vprefix; unused with n_prefix 0), and
+ * over the sequence's own n_keys[s] keys, at positions n_prefix + j. The query is at the
+ * last of these positions. n_keys is a device array; a length outside 0 .. max_seq counts as
+ * the nearer of the two. A query that sees no key gets zeros. options may be NULL.
+ * q and out must not overlap. Its scratch is the library's (see uaii_hip_gemm). */
+UAII_HIP_API int uaii_hip_attention_batch(const float* q, int64_t ldq, int64_t n_seq, const void* kcache,
+                                          const void* vcache, int kv_type, int64_t max_seq, const int32_t* n_keys,
+                                          const void* kprefix, const void* vprefix, int64_t prefix_seq,
+                                          int64_t n_prefix, int n_heads, int n_kv_heads, int head_dim,
+                                          const uaii_hip_score_options* options, float* out, int64_t ldo,
+                                          void* stream);
+/* Attention of m queries at positions p0 .. p0 + m - 1 over one sequence's cache, which holds
+ * the keys 0 .. p0 + m - 1. The query at i sees the keys j <= i and, wherever it is, the keys
+ * j < bidirectional (0: causal; at most p0 + m); of these only j >= first_key[i - p0], where
+ * that device array of m is given (packed documents; padding sees nothing behind its own
+ * position), and those in the options' window. A query that sees no key gets zeros.
+ * q and out must not overlap. */
+UAII_HIP_API int uaii_hip_attention_prompt(const float* q, int64_t ldq, int64_t m, const void* kcache,
+                                           const void* vcache, int kv_type, int64_t max_seq, int64_t p0,
+                                           int64_t bidirectional, const int32_t* first_key, int n_heads,
+                                           int n_kv_heads, int head_dim, const uaii_hip_score_options* options,
+                                           float* out, int64_t ldo, void* stream);
 
 /* ---- timing (HIP events on `stream`) ---------------------------------------- */
 /* Average device time of `iters` back-to-back uaii_hip_gemv launches, in ms. */

@@ -88,6 +88,20 @@ class SampleParams(C.Structure):
                 ("has_seed", C.c_int)]
 
 
+# cache types of uaii_hip_kv_append_batch and the attentions over them (include/uaii_hip.h)
+KV_F32, KV_F16, KV_Q8 = 0, 1, 2
+
+
+class ScoreOptions(C.Structure):
+    """uaii_hip_score_options (include/uaii_hip.h)."""
+    _fields_ = [("struct_size", C.c_uint32), ("scale", C.c_float), ("softcap", C.c_float),
+                ("slopes", C.c_void_p), ("window", C.c_int64)]
+
+    def __init__(self, scale=0.0, softcap=0.0, slopes=None, window=0):
+        """slopes: a device pointer (c_void_p or address) of one float a query head, or None."""
+        super().__init__(C.sizeof(ScoreOptions), scale, softcap, slopes, window)
+
+
 def sample_params(temperature=0.0, top_p=1.0, top_k=0, repetition_penalty=1.0, seed=None):
     p = SampleParams()
     lib().uaii_sample_params_init(C.byref(p))
@@ -214,6 +228,15 @@ def lib() -> C.CDLL:
         "uaii_hip_gelu": (C.c_int, [vp, vp, i64, vp]),
         "uaii_hip_embed": (C.c_int, [vp, vp, i64, vp, vp]),
         "uaii_hip_kv_append": (C.c_int, [vp, vp, vp, vp, i64, i64, C.c_int, i64, i64, C.c_int, vp]),
+        "uaii_hip_kv_cache_bytes": (i64, [C.c_int, C.c_int, i64, C.c_int]),
+        "uaii_hip_kv_append_batch": (C.c_int, [vp, vp, i64, vp, vp, C.c_int, i64, i64, C.c_int, C.c_int, i64,
+                                               i64, vp, vp]),
+        "uaii_hip_kv_read": (C.c_int, [vp, C.c_int, i64, i64, C.c_int, C.c_int, i64, i64, vp, vp, i64, vp]),
+        "uaii_hip_score_options_init": (None, [C.POINTER(ScoreOptions)]),
+        "uaii_hip_attention_batch": (C.c_int, [vp, i64, i64, vp, vp, C.c_int, i64, vp, vp, vp, i64, i64, C.c_int,
+                                               C.c_int, C.c_int, C.POINTER(ScoreOptions), vp, i64, vp]),
+        "uaii_hip_attention_prompt": (C.c_int, [vp, i64, i64, vp, vp, C.c_int, i64, i64, i64, vp, C.c_int, C.c_int,
+                                                C.c_int, C.POINTER(ScoreOptions), vp, i64, vp]),
         "uaii_backend_create": (C.c_int, [C.c_char_p, C.c_int, C.POINTER(vp)]),
         "uaii_backend_destroy": (None, [vp]),
         "uaii_backend_initialize": (C.c_int, [vp]),
