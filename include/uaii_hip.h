@@ -222,7 +222,8 @@ UAII_HIP_API int uaii_hip_attention_prefill(const float* q, const void* kcache,
  * scales: a value is (byte - 128) * scale, a head's row having one scale, max |x| / 127
  * (the next lower number where 127 of it would pass the end of f32). Rows with an infinity or a NaN read back as NaN. A batch's caches lie one behind the
  * other, sequence s at s * uaii_hip_kv_cache_bytes. Caches are 16-byte aligned; head_dim
- * is a multiple of 16 up to 256. */
+ * is a multiple of 16 up to 256; max_seq, and a prefix and max_seq together, are at most 2^30
+ * positions. */
 #define UAII_HIP_KV_F32 0
 #define UAII_HIP_KV_F16 1
 #define UAII_HIP_KV_Q8 2

@@ -23,7 +23,7 @@ def test_cache_bytes():
     assert L.uaii_hip_kv_cache_bytes(KV_Q8, 8, 100, 64) == 8 * 100 * 68
     assert L.uaii_hip_kv_cache_bytes(KV_Q8, 1, 7, 16) == 144  # 140 bytes, to the next 16
     for bad in [(3, 8, 100, 64), (-1, 8, 100, 64), (KV_Q8, 0, 100, 64), (KV_Q8, 8, 0, 64), (KV_Q8, 8, 100, 0), (KV_Q8, 8, 100, 72),
-                (KV_Q8, 8, 100, 272), (KV_Q8, 8, 1 << 31, 64), (KV_Q8, 65536, 100, 64)]:
+                (KV_Q8, 8, 100, 272), (KV_Q8, 8, (1 << 30) + 1, 64), (KV_Q8, 65536, 100, 64)]:
         assert L.uaii_hip_kv_cache_bytes(*bad) == -1, bad
 
 
@@ -42,7 +42,7 @@ def rows_call(append, **kw):
 @pytest.mark.parametrize("append", [True, False])
 @pytest.mark.parametrize("bad", [dict(k=None), dict(kc=None), dict(kc=4 * A + 8), dict(k=A + 2), dict(past=6 * A + 2), dict(t=3),
                                  dict(t=-1), dict(n=-1), dict(rows=-1), dict(kv=0), dict(hd=24), dict(hd=0), dict(hd=512), dict(seq=0),
-                                 dict(seq=1 << 31), dict(ld=511), dict(p0=-1), dict(p0=101), dict(past=None, p0=98),
+                                 dict(seq=(1 << 30) + 1), dict(ld=511), dict(p0=-1), dict(p0=101), dict(past=None, p0=98),
                                  dict(rows=1 << 32), dict(n=1 << 31), dict(n=1 << 16, rows=1 << 13)], ids=str)
 def test_rows_refused(append, bad):
     assert rows_call(append, **bad) == REFUSED
@@ -83,7 +83,7 @@ def short_options():
 @pytest.mark.parametrize("batch", [True, False])
 @pytest.mark.parametrize("bad", [dict(q=None), dict(out=None), dict(kc=None), dict(vc=None), dict(kc=4 * A + 8), dict(vc=5 * A + 2), dict(q=A + 1),
                                  dict(out=16 * A + 2), dict(ldq=2047), dict(ldo=2047), dict(n=-1), dict(n=1 << 31), dict(t=5), dict(seq=0),
-                                 dict(seq=1 << 31), dict(heads=0), dict(heads=33), dict(heads=65536 * 8), dict(kv=0), dict(hd=65), dict(hd=0),
+                                 dict(seq=(1 << 30) + 1), dict(heads=0), dict(heads=33), dict(heads=65536 * 8), dict(kv=0), dict(hd=65), dict(hd=0),
                                  dict(hd=288), dict(out=A), dict(out=A + 4 * 2047), dict(out=A - 4 * 2048), dict(opt=dict(softcap=-1.0)),
                                  dict(opt=dict(softcap=float("nan"))), dict(opt=dict(softcap=float("inf"))), dict(opt=dict(scale=float("inf"))),
                                  dict(opt=dict(window=-1)), dict(opt=dict(slopes=ctypes.c_void_p(A + 2))), dict(opt=short_options())],
@@ -93,7 +93,7 @@ def test_attention_refused(batch, bad):
 
 
 @pytest.mark.parametrize("bad", [dict(lens=None), dict(lens=6 * A + 1), dict(prefix=-1), dict(kp=None), dict(vp=None), dict(kp=7 * A + 8),
-                                 dict(prefix=51), dict(prefix=(1 << 31) - 100, pre_seq=(1 << 31) - 1), dict(pre_seq=1 << 31)], ids=str)
+                                 dict(prefix=51), dict(prefix=(1 << 30) - 99, pre_seq=1 << 30), dict(pre_seq=(1 << 30) + 1)], ids=str)
 def test_batch_refused(bad):
     assert attn_call(True, **bad) == REFUSED
 

@@ -1,83 +1,681 @@
-// batch_attn.hip — attention over the caches of a batch, one block a (row, query head).
-#include "kv_cache.h"
+// batch_attn.hip — attention of one query for each sequence of a batch over the
+// sequence's own keys, and the join of partial results.
+//
+// Lengths are on the device, so the host cannot cut the work to them. Each (sequence, kv
+// head) is cut into units of 128 keys and the units of the whole batch, in order, are
+// dealt out evenly to a grid that just fills the device: a block works through the runs of
+// units that fall to it, writes a finished head's rows to the output at once, and leaves
+// the partial results of its first and last run, where a head goes on in another block,
+// to the join.
+#include "seq_attn.h"
+
+#include <algorithm>
 
 namespace uaii_hip {
 namespace {
 
-__device__ inline float cache_value(const uint8_t* base, int type, int n_kv, int64_t max_seq, int hd, int h, int64_t j, int d) {
-  const int64_t row = (int64_t)h * max_seq + j;
-  if (type == KV_F32) return reinterpret_cast<const float*>(base)[row * hd + d];
-  if (type == KV_F16) return (float)reinterpret_cast<const _Float16*>(base)[row * hd + d];
-  const float s = reinterpret_cast<const float*>(base + (int64_t)n_kv * max_seq * hd)[row];
-  return (float)((int)base[row * hd + d] - 128) * s;
+constexpr int UNIT = 128;  // keys
+
+struct BatchArgs {
+  SeqAttnArgs a;
+  int G, groups;       // query heads of a kv head, and its row groups of RC
+  float* slots;        // [2 blocks][RC][part_stride]: a block's first and last run
+  float* whole;        // [n_seq * n_kv * groups][RC][part_stride], with a prefix only
+  int* info;           // first unit of each (sequence, kv head, group), then the units of all
+  const float* pre;    // partials over the prefix (RowsAttnArgs::part)
+  int pre_splits, blocks;
+};
+
+__device__ inline f4_t mfma32(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ inline f4_t mfma16(h4_t a, h4_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
+__device__ inline f4_t mfma4(float a, float b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// Weight of a partial with running maximum m and sum l; a sum that is NaN stays in.
+__device__ inline float weight_of(float m, float l, float M) {
+  if (l != l) return 1.0f;
+  return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
 }
 
-__global__ void __launch_bounds__(256) k_seq_attn(SeqAttnArgs a) {
-  __shared__ float q_s[256], p_s[256], red[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t r = blockIdx.x;
-  const int h = blockIdx.y, kh = h / (a.n_heads / a.n_kv);
-  const bool batch = a.n_keys != nullptr;
-  const int pre = batch ? a.n_prefix : 0;
-  int pos, hi, lo = 0;
-  if (batch) {
-    const int n = (int)min((int64_t)max(a.n_keys[r], 0), a.max_seq);
-    pos = pre + n - 1;
-    hi = pre + n;
+struct Span {
+  int n, lo;  // keys lo .. n - 1 of the sequence
+  __device__ int units() const { return (n - lo + UNIT - 1) / UNIT; }
+};
+
+__device__ inline Span span_of(const SeqAttnArgs& a, int64_t s) {
+  Span p;
+  p.n = (int)min((int64_t)max(a.n_keys[s], 0), a.max_seq);
+  p.lo = a.window ? max(0, p.n - a.window) : 0;
+  return p;
+}
+
+template <int N>
+__device__ inline void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(p);
+    w[0] = x.x, w[1] = x.y;
   } else {
-    pos = a.p0 + (int)r;
-    hi = max(pos + 1, a.bidir);
-    if (a.first) lo = max(0, a.first[r]);
-  }
-  if (a.window) lo = max(lo, pos - a.window + 1);
-  const uint8_t* kc = a.kc + (batch ? r * a.seq_bytes : 0);
-  const uint8_t* vc = a.vc + (batch ? r * a.seq_bytes : 0);
-  if (tid < a.hd) q_s[tid] = a.q[r * a.ldq + (int64_t)h * a.hd + tid] * a.scale;
-  __syncthreads();
-  float m = -INFINITY, l = 0.0f, o = 0.0f;
-  for (int64_t t0 = lo; t0 < hi; t0 += 256) {
-    const int64_t j = t0 + tid;
-    float s = -INFINITY;
-    if (j < hi) {
-      float dot = 0.0f;
-      for (int d = 0; d < a.hd; ++d)
-        dot += q_s[d] * (j < pre ? cache_value(a.kp, a.type, a.n_kv, a.pre_seq, a.hd, kh, j, d)
-                                 : cache_value(kc, a.type, a.n_kv, a.max_seq, a.hd, kh, j - pre, d));
-      s = a.cap > 0.0f ? a.cap * tanhf(dot / a.cap) : dot;
-      if (a.slopes) s -= a.slopes[h] * (float)abs((int)(pos - j));
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const u4_t x = *reinterpret_cast<const u4_t*>(p + 4 * i);
+      w[i] = x[0], w[i + 1] = x[1], w[i + 2] = x[2], w[i + 3] = x[3];
     }
-    float mx = wave_max(s);
-    if (lane == 0) red[wave] = mx;
+  }
+}
+
+// Rows of a group: the matrix op has 16 columns. With up to 8 rows (PACK) the f16 types put
+// the high halves of q, and of the probabilities, into columns 0-7 and the low halves
+// beside them into 8-15, half the matrix ops.
+constexpr int rows_of(bool pack) { return pack ? 8 : 16; }
+
+template <int TYPE, int HD, bool PACK>
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs b) {
+  constexpr int NW = 4;
+  constexpr int ES = TYPE == KV_F32 ? 4 : TYPE == KV_F16 ? 2 : 1;
+  constexpr int NS = TYPE == KV_F32 || (TYPE == KV_F16 && HD == 256) ? 1 : 2;  // 16-key subtiles of a tile
+  constexpr int KT = 16 * NS;
+  constexpr int RC = rows_of(PACK);
+  constexpr int E = HD / 16;                // value dims of a lane
+  constexpr int KW = HD / 4 * ES / 4;       // words of a lane's part of a key
+  constexpr int VW = E * ES / 4;            // words of its part of a value row
+  constexpr int NC = HD / 32;               // 32-dim chunks of a score
+  constexpr int QH = TYPE == KV_F32 ? HD / 8 : PACK ? NC : 2 * NC;  // fragments of q, 1 KB each (f32: 256 B each, by fours)
+  constexpr bool SC = TYPE == KV_Q8;
+  constexpr int WS = HD + 4;                // row of the waves' outputs
+  __shared__ __attribute__((aligned(16))) uint32_t qf[TYPE == KV_F32 ? HD / 4 * 64 : QH * 256];
+  __shared__ __attribute__((aligned(16))) float wo[NW][RC][WS];
+  __shared__ __attribute__((aligned(16))) float sc[NW][64];
+  __shared__ float wm[NW][16], wl[NW][16], qtop[16];
+  __shared__ int scan[NW], found[2];
+
+  const SeqAttnArgs& a = b.a;
+  const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int H = a.n_kv * b.groups;
+  const int n_seq = (int)a.rows;
+
+  // ---- this block's units [u, u1) of the batch's, and the sequence where they begin
+  int total;
+  {
+    const int per = (n_seq + 255) / 256, s0 = min(n_seq, tid * per), s1 = min(n_seq, s0 + per);
+    int mine = 0;
+    for (int s = s0; s < s1; ++s) mine += span_of(a, s).units();
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int x = __shfl_up(incl, o, 64);
+      incl += lane >= o ? x : 0;
+    }
+    if (lane == 63) scan[wave] = incl;
     __syncthreads();
-    const float mnew = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
-    const float p = s == -INFINITY ? 0.0f : expf(s - mnew);
-    p_s[tid] = p;
-    const float sum = wave_sum(p);
+    int below = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      below += w < wave ? scan[w] : 0;
+      total += scan[w];
+    }
+    total *= H;
+    if (blockIdx.x == 0 && tid == 0) b.info[(int64_t)n_seq * H] = total;
+    const int at = (int)((int64_t)total * blockIdx.x / max(1, min(b.blocks, total)));
+    int before = below + incl - mine;  // units of a head's worth of the sequences before s0
+    if (before * H <= at && at < (before + mine) * H) {
+      int s = s0;
+      for (;; ++s) {
+        const int n = span_of(a, s).units();
+        if (at < (before + n) * H) break;
+        before += n;
+      }
+      found[0] = s;
+      found[1] = before;
+    }
     __syncthreads();
-    if (lane == 0) red[wave] = sum;
-    __syncthreads();
-    const float alpha = m == -INFINITY ? 0.0f : expf(m - mnew);
-    l = l * alpha + (red[0] + red[1] + red[2] + red[3]);
-    m = mnew;
-    o *= alpha;
-    if (tid < a.hd) {
-      const int n = (int)min((int64_t)256, hi - t0);
-      for (int i = 0; i < n; ++i) {
-        const int64_t jj = t0 + i;
-        o += p_s[i] * (jj < pre ? cache_value(a.vp, a.type, a.n_kv, a.pre_seq, a.hd, kh, jj, tid)
-                                : cache_value(vc, a.type, a.n_kv, a.max_seq, a.hd, kh, jj - pre, tid));
+  }
+  const int blocks = min(b.blocks, total);  // each has a unit at least
+  if ((int)blockIdx.x >= blocks) return;
+  int u = (int)((int64_t)total * blockIdx.x / blocks);
+  const int u1 = (int)((int64_t)total * (blockIdx.x + 1) / blocks);
+  int s = __builtin_amdgcn_readfirstlane(found[0]), base = __builtin_amdgcn_readfirstlane(found[1]) * H;
+
+  const bool capped = a.cap > 0.0f, sloped = a.slopes != nullptr;
+  const int crow = PACK ? col & 7 : col;  // the lane's row of the group
+  const bool low = PACK && col >= 8;      // it works on the low halves
+
+  while (u < u1) {
+    Span sp = span_of(a, s);
+    int units = sp.units();
+    while (units == 0) {  // sequences with no keys
+      if (++s >= n_seq) return;
+      sp = span_of(a, s);
+      units = sp.units();
+    }
+    const int hx = (u - base) / units, uu = (u - base) % units, ue = min(units, uu + u1 - u);
+    const int kvh = hx / b.groups, head0 = kvh * b.G + hx % b.groups * RC;
+    const int rows = min(RC, b.G - hx % b.groups * RC);
+    const int k0 = sp.lo + UNIT * uu, k1 = min(sp.n, sp.lo + UNIT * ue);
+    if (uu == 0 && tid == 0) b.info[(int64_t)s * H + hx] = u;
+
+    const int64_t first = (int64_t)kvh * a.max_seq;
+    const uint8_t* kbase = a.kc + (int64_t)s * a.seq_bytes;
+    const uint8_t* vbase = a.vc + (int64_t)s * a.seq_bytes;
+    const float* kscale = reinterpret_cast<const float*>(kbase + (int64_t)a.n_kv * a.max_seq * a.hd) + first;  // KV_Q8
+    const float* vscale = reinterpret_cast<const float*>(vbase + (int64_t)a.n_kv * a.max_seq * a.hd) + first;
+    kbase += first * a.hd * ES;
+    vbase += first * a.hd * ES;
+
+    struct Tile {
+      uint32_t k[NS][KW], v[NS][4][VW];
+      float f;
+    } t0, t1;
+    // keys behind the last repeat it and are masked; dims behind the row's end repeat its
+    // last piece, which meets zeros of q or goes to outputs that are not stored
+    auto load = [&](int t, Tile& x) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const uint8_t* kr = kbase + (int64_t)min(t + 16 * i + col, k1 - 1) * a.hd * ES;
+#pragma unroll
+        for (int w = 0; w < KW; w += 4) {
+          constexpr int P = 16 / ES;
+          const int d = min(g * (HD / 4) + w / 4 * P, a.hd - P);
+          const u4_t y = *reinterpret_cast<const u4_t*>(kr + d * ES);
+          x.k[i][w] = y[0], x.k[i][w + 1] = y[1], x.k[i][w + 2] = y[2], x.k[i][w + 3] = y[3];
+        }
+      }
+      const int d = min(col * E, a.hd - E);
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          load_words<VW>(vbase + ((int64_t)min(t + 16 * i + 4 * g + r, k1 - 1) * a.hd + d) * ES, x.v[i][r]);
+      if constexpr (SC) x.f = (lane < 32 ? kscale : vscale)[min(t + (lane & 31), k1 - 1)];
+    };
+
+    const int step = NW * KT, mine = k0 + wave * KT;
+    if (mine < k1) load(mine, t0);
+
+    // ---- q into fragments in LDS
+    const float* qrow = a.q + (int64_t)s * a.ldq + (int64_t)head0 * a.hd;
+    if constexpr (TYPE != KV_F32) {
+      // 16 lanes a row: its largest magnitude, for the power of two that it is scaled by
+      const int r = tid >> 4;
+      float top = 0.0f;
+      if (r < rows)
+        for (int d = tid & 15; d < a.hd; d += 16) top = fmaxf(top, fabsf(qrow[(int64_t)r * a.hd + d] * a.scale));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+      if ((tid & 15) == 0) qtop[r] = top;
+      __syncthreads();
+      for (int x = tid; x < NC * 64; x += 256) {
+        const int c = x >> 6, ln = x & 63, cc = ln & 15, d0 = (ln >> 4) * (HD / 4) + 8 * c, rr = PACK ? cc & 7 : cc;
+        const float up = pow2i(row_exponent(qtop[rr]));
+        h8_t hi, lo;
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+          // bytes of a word pair up as 0 and 2, 1 and 3
+          const int ka = TYPE == KV_Q8 ? (k & 4) + (k >> 1 & 1) : k, kb = TYPE == KV_Q8 ? ka + 2 : k + 1;
+          const bool in = rr < rows && d0 < a.hd;
+          const float va = in ? qrow[(int64_t)rr * a.hd + d0 + ka] * a.scale * up : 0.0f;
+          const float vb = in ? qrow[(int64_t)rr * a.hd + d0 + kb] * a.scale * up : 0.0f;
+          h2_t p, q;
+          split2(va, vb, p, q);
+          hi[k] = p.x, hi[k + 1] = p.y, lo[k] = q.x, lo[k + 1] = q.y;
+        }
+        h8_t* to = reinterpret_cast<h8_t*>(qf);
+        if constexpr (PACK) {
+          to[x] = cc >= 8 ? lo : hi;
+        } else {
+          to[x] = hi;
+          to[NC * 64 + x] = lo;
+        }
+      }
+    } else {
+      for (int x = tid; x < HD / 4 * 64; x += 256) {
+        const int ln = x >> 2 & 63, d = (ln >> 4) * (HD / 4) + (x >> 8) * 4 + (x & 3), rr = ln & 15;
+        qf[x] = __float_as_uint(rr < rows && d < a.hd ? qrow[(int64_t)rr * a.hd + d] * a.scale : 0.0f);
       }
     }
     __syncthreads();
+    const float unit = TYPE == KV_F32 ? 1.0f : pow2i(-row_exponent(qtop[crow])) * (SC ? kQ8Unit : 1.0f);
+    const float to_cap = capped ? unit / a.cap : 0.0f;
+    const float mul = (capped ? a.cap : unit) * kLog2e;  // scores in base 2
+    const float slope = sloped && crow < rows ? a.slopes[head0 + crow] * kLog2e : 0.0f;
+
+    f4_t o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    // as in rows_attn.hip: probabilities are 2^(y - m + 10) / D
+    float m = -INFINITY, l = 0.0f, D = SC ? 0x1p-60f : 1.0f, lgD = SC ? -60.0f : 0.0f;
+
+    auto tile = [&](int t, const Tile& x) __attribute__((always_inline)) {
+      f4_t y[NS];
+      if constexpr (SC) {
+        sc[wave][lane] = x.f;
+        const float f = lane >= 32 ? x.f : 0.0f;
+        if (__any(f > D && f < INFINITY)) {
+          const float top = wave_max_dpp(f < INFINITY ? f : 0.0f);
+          const int e = min(126, (int)((__float_as_uint(top) >> 23) & 0xff) - 126);
+          const float Dnew = pow2i(e), beta = D / Dnew;
+          D = Dnew;
+          lgD = (float)e;
+          l *= beta;
+#pragma unroll
+          for (int k = 0; k < E; ++k) o[k] *= beta;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NS; ++i) y[i] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (TYPE == KV_F32) {
+#pragma unroll
+        for (int w = 0; w < KW; w += 4) {
+          const f4_t q = reinterpret_cast<const f4_t*>(qf)[w / 4 * 64 + lane];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y[0] = mfma4(__uint_as_float(x.k[0][w + k]), q[k], y[0]);
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          const h8_t q0 = reinterpret_cast<const h8_t*>(qf)[c * 64 + lane];
+          h8_t q1;
+          if constexpr (!PACK) q1 = reinterpret_cast<const h8_t*>(qf)[(NC + c) * 64 + lane];
+#pragma unroll
+          for (int i = 0; i < NS; ++i) {
+            h8_t kf;
+            if constexpr (TYPE == KV_F16) {
+              kf = __builtin_bit_cast(h8_t, (u4_t{x.k[i][4 * c], x.k[i][4 * c + 1], x.k[i][4 * c + 2], x.k[i][4 * c + 3]}));
+            } else {
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                const uint32_t z = x.k[i][2 * c + w];
+                const h2_t p = q8_pair(z & 0x00ff00ffu), q = q8_pair(__builtin_amdgcn_perm(0, z, 0x0c030c01));
+                kf[4 * w] = p.x, kf[4 * w + 1] = p.y, kf[4 * w + 2] = q.x, kf[4 * w + 3] = q.y;
+              }
+            }
+            y[i] = mfma32(kf, q0, y[i]);
+            if constexpr (!PACK) y[i] = mfma32(kf, q1, y[i]);
+          }
+        }
+        if constexpr (PACK) {
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[i][r] += dpp_mov<0x128>(y[i][r]);  // row_ror 8: the other half's column
+        }
+      }
+      // element r of y[i]: key t + 16 i + 4 g + r
+      f4_t vf[NS];
+      if constexpr (SC) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          y[i] *= *reinterpret_cast<const f4_t*>(&sc[wave][16 * i + 4 * g]);
+          vf[i] = *reinterpret_cast<const f4_t*>(&sc[wave][32 + 16 * i + 4 * g]);
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+      float y_of = mul;
+      if (capped) {
+        float far = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            y[i][r] *= to_cap;
+            far = fmaxf(far, fabsf(y[i][r]));
+          }
+        const bool some_far = __any(!(far < 0.9f));
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float z = y[i][r];
+            y[i][r] = tanh_near(z);
+            if (some_far) y[i][r] = fabsf(z) < 0.9f ? y[i][r] : tanh_far(z);
+          }
+      }
+      if (sloped) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[i][r] = fmaf(y[i][r], mul, -slope * (float)(sp.n - 1 - (t + 16 * i + 4 * g + r)));
+        y_of = 1.0f;
+      }
+      if (t + KT > k1) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[i][r] = t + 16 * i + 4 * g + r < k1 ? y[i][r] : -INFINITY;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) top = fmaxf(top, y[i][r]);
+      top *= y_of;
+      if (__any(top > m + 4.0f)) {
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float mnew = fmaxf(m, top);
+        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mnew);
+        m = mnew;
+        l *= alpha;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] *= alpha;
+      }
+      const float ref = (m == -INFINITY ? 0.0f : m) + lgD - 10.0f;
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          y[i][r] = __builtin_amdgcn_exp2f(fmaf(y[i][r], y_of, -ref));
+          l += y[i][r];
+        }
+      if constexpr (SC) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) y[i] *= vf[i];
+      }
+      // O^T += V^T . P^T: the lane's probabilities are the operand as they lie, the keys
+      // 4 g + r of a subtile being its k index; a value's dims are E col + e
+      if constexpr (TYPE == KV_F32) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] = mfma4(__uint_as_float(x.v[0][r][e]), y[0][r], o[e]);
+      } else {
+        h4_t p0[NS], p1[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; r += 2) {
+            h2_t hi, lo;
+            split2(y[i][r], y[i][r + 1], hi, lo);
+            if constexpr (PACK) {
+              const uint32_t z = low ? __builtin_bit_cast(uint32_t, lo) : __builtin_bit_cast(uint32_t, hi);
+              hi = __builtin_bit_cast(h2_t, z);
+            }
+            p0[i][r] = hi.x, p0[i][r + 1] = hi.y;
+            p1[i][r] = lo.x, p1[i][r + 1] = lo.y;
+          }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          h4_t vv[NS];
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; r += 2) {
+              h2_t z;
+              if constexpr (TYPE == KV_F16) {
+                z = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(x.v[i][r + 1][e / 2], x.v[i][r][e / 2], e & 1 ? 0x07060302 : 0x05040100));
+              } else {
+                z = q8_pair(__builtin_amdgcn_perm(x.v[i][r + 1][e / 4], x.v[i][r][e / 4], 0x0c040c00 + (e & 3) * 0x00010001));
+              }
+              vv[i][r] = z.x, vv[i][r + 1] = z.y;
+            }
+          if constexpr (NS == 2) {
+            const h8_t v8 = __builtin_shufflevector(vv[0], vv[NS - 1], 0, 1, 2, 3, 4, 5, 6, 7);
+            o[e] = mfma32(v8, __builtin_shufflevector(p0[0], p0[NS - 1], 0, 1, 2, 3, 4, 5, 6, 7), o[e]);
+            if constexpr (!PACK) o[e] = mfma32(v8, __builtin_shufflevector(p1[0], p1[NS - 1], 0, 1, 2, 3, 4, 5, 6, 7), o[e]);
+          } else {
+            o[e] = mfma16(vv[0], p0[0], o[e]);
+            if constexpr (!PACK) o[e] = mfma16(vv[0], p1[0], o[e]);
+          }
+        }
+      }
+    };
+
+    for (int t = mine; t < k1; t += 2 * step) {
+      if (t + step < k1) load(t + step, t1);
+      tile(t, t0);
+      if (t + step >= k1) break;
+      if (t + 2 * step < k1) load(t + 2 * step, t0);
+      tile(t + step, t1);
+    }
+
+    // ---- the waves' results together
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    const float back = D * 0x1p-10f, back_o = SC ? back * kQ8Unit : back;
+    if constexpr (PACK) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[e][r] += dpp_mov<0x128>(o[e][r]);
+    }
+    if (!low) {
+      if (g == 0) wm[wave][crow] = m, wl[wave][crow] = l * back;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < E; e += 4)
+          *reinterpret_cast<f4_t*>(&wo[wave][crow][(4 * g + r) * E + e]) = f4_t{o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]} * back_o;
+    }
+    __syncthreads();
+    const bool complete = uu == 0 && ue == units;
+    const int64_t stride = part_stride(a.hd);
+    const bool direct = complete && b.pre_splits == 0;
+    float* part = complete ? b.whole + ((int64_t)s * H + hx) * RC * stride : b.slots + (2 * (int64_t)blockIdx.x + (uu == 0)) * RC * stride;
+    for (int x = tid; x < rows * (a.hd / 4); x += 256) {
+      const int r = x / (a.hd / 4), d = x % (a.hd / 4) * 4;
+      float M = -INFINITY, den = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) M = fmaxf(M, wm[w][r]);
+      f4_t acc = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float f = weight_of(wm[w][r], wl[w][r], M);
+        acc += f * *reinterpret_cast<const f4_t*>(&wo[w][r][d]);
+        den += f * wl[w][r];
+      }
+      if (direct) {
+        const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+        *reinterpret_cast<f4u_t*>(a.out + (int64_t)s * a.ldo + (int64_t)(head0 + r) * a.hd + d) = acc * inv;
+      } else {
+        *reinterpret_cast<f4_t*>(part + r * stride + d) = acc;
+        if (d == 0) part[r * stride + a.hd] = M, part[r * stride + a.hd + 1] = den;
+      }
+    }
+    __syncthreads();
+
+    u += ue - uu;
+    if (ue == units && hx == H - 1) {
+      ++s;
+      base = u;
+    }
   }
-  if (tid < a.hd) a.out[r * a.ldo + (int64_t)h * a.hd + tid] = lo < hi ? o / l : 0.0f;
+}
+
+// Partial results of a row into its output: block (row, query head), the waves taking
+// partials in turn.
+struct JoinArgs {
+  SeqAttnArgs a;
+  int G, rc, groups, blocks;
+  const float* slots;
+  const float* whole;
+  const int* info;       // null: no own keys (prompt rows)
+  const float* part;     // [splits][n_kv][rows * G][part_stride]
+  int splits;
+};
+
+__global__ void __launch_bounds__(256) k_attn_join(JoinArgs j) {
+  __shared__ float wm[4], wl[4];
+  __shared__ __attribute__((aligned(16))) float wo[4][256];
+  const SeqAttnArgs& a = j.a;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = (int)(blockIdx.x / (unsigned)a.n_heads), head = (int)(blockIdx.x % (unsigned)a.n_heads);
+  const int kvh = head / j.G, gr = head % j.G, H = a.n_kv * j.groups;
+  const int64_t stride = part_stride(a.hd);
+  // the row's own partials: those of blocks b0 .. b1, or one in `whole`
+  int own = 0, b0 = 0;
+  const float* at = nullptr;
+  if (j.info) {
+    const Span sp = span_of(a, row);
+    const int units = sp.units();
+    if (units > 0) {
+      const int hx = kvh * j.groups + gr / j.rc;
+      const int64_t first = j.info[(int64_t)row * H + hx], total = j.info[a.rows * H];
+      // block of unit u: the last one whose first unit, total b / blocks, is not behind it
+      const int64_t blocks = min((int64_t)j.blocks, total);
+      b0 = (int)(((first + 1) * blocks - 1) / total);
+      own = (int)(((first + units) * blocks - 1) / total) - b0 + 1;
+      if (own == 1 && j.splits == 0) return;  // written
+      at = own == 1 ? j.whole + ((int64_t)row * H + hx) * j.rc * stride : j.slots + (2 * (int64_t)b0 + 1) * j.rc * stride;
+      at += gr % j.rc * stride;
+    }
+  }
+  const int64_t R = a.rows * j.G;
+  const float* pre = j.part + ((int64_t)kvh * R + (int64_t)row * j.G + gr) * stride;
+  auto part_of = [&](int i) -> const float* {
+    if (i >= own) return pre + (int64_t)(i - own) * a.n_kv * R * stride;
+    return i == 0 ? at : at + (2 * (int64_t)i - 1) * j.rc * stride;  // the blocks behind b0: their first run
+  };
+  const int n = own + j.splits, d = min(4 * lane, a.hd - 4);
+  float m = -INFINITY, l = 0.0f;
+  f4_t o = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i0 = wave; i0 < n; i0 += 16) {
+    float mi[4], li[4];
+    f4_t oi[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float* p = part_of(min(i0 + 4 * k, n - 1));
+      mi[k] = p[a.hd], li[k] = p[a.hd + 1];
+      oi[k] = *reinterpret_cast<const f4_t*>(p + d);
+    }
+    float M = m;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) M = i0 + 4 * k < n ? fmaxf(M, mi[k]) : M;
+    const float keep = weight_of(m, l, M);
+    l *= keep;
+    o *= keep;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (i0 + 4 * k >= n) continue;
+      const float f = weight_of(mi[k], li[k], M);
+      l += f * li[k];
+      o += f * oi[k];
+    }
+    m = M;
+  }
+  if (lane == 0) wm[wave] = m, wl[wave] = l;
+  *reinterpret_cast<f4_t*>(&wo[wave][4 * lane]) = o;
+  __syncthreads();
+  if (wave != 0 || 4 * lane >= a.hd) return;
+  float M = -INFINITY, den = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) M = fmaxf(M, wm[w]);
+  f4_t acc = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float f = weight_of(wm[w], wl[w], M);
+    den += f * wl[w];
+    acc += f * *reinterpret_cast<const f4_t*>(&wo[w][4 * lane]);
+  }
+  const float inv = den == 0.0f ? 0.0f : 1.0f / den;
+  *reinterpret_cast<f4u_t*>(a.out + (int64_t)row * a.ldo + (int64_t)head * a.hd + 4 * lane) = acc * inv;
+}
+
+template <int TYPE, int HD, bool PACK>
+hipError_t go(BatchArgs& b, hipStream_t s) {
+  UAII_LAUNCH((k_batch_attn<TYPE, HD, PACK>), dim3((unsigned)b.blocks), dim3(256), 0, s, b);
+  return hipGetLastError();
+}
+
+template <int TYPE>
+hipError_t by_width(BatchArgs& b, bool pack, hipStream_t s) {
+  if constexpr (TYPE != KV_F32) {
+    if (pack) {
+      if (b.a.hd <= 64) return go<TYPE, 64, true>(b, s);
+      if (b.a.hd <= 128) return go<TYPE, 128, true>(b, s);
+      return go<TYPE, 256, true>(b, s);
+    }
+  }
+  if (b.a.hd <= 64) return go<TYPE, 64, false>(b, s);
+  if (b.a.hd <= 128) return go<TYPE, 128, false>(b, s);
+  return go<TYPE, 256, false>(b, s);
+}
+
+struct Plan {
+  int G, groups, rc, blocks, splits;
+  bool pack;
+  RowsAttnArgs rows;
+  size_t part, slots, whole, info;  // bytes of the scratch's parts
+  size_t bytes() const { return part + slots + whole + info; }
+};
+
+size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
+
+Plan plan_of(const SeqAttnArgs& a) {
+  Plan p{};
+  p.G = a.n_heads / a.n_kv;
+  const size_t row = (size_t)part_stride(a.hd) * 4;
+  p.rows.a = a;
+  p.rows.G = p.G;
+  p.rows.R = a.rows * p.G;
+  if (!a.n_keys) {
+    p.rows.splits = rows_attn_splits(p.rows, (int64_t)a.p0 + a.rows);
+    p.splits = p.rows.splits > 1 ? p.rows.splits : 0;
+  } else {
+    p.pack = a.type != KV_F32 && p.G <= 8;
+    p.rc = rows_of(p.pack);
+    p.groups = (p.G + p.rc - 1) / p.rc;
+    const int64_t units = a.rows * a.n_kv * p.groups * ((a.max_seq + UNIT - 1) / UNIT);
+    p.blocks = (int)std::min<int64_t>(units, (int64_t)device_cus() * 2);
+    p.slots = pad256(2 * (size_t)p.blocks * p.rc * row);
+    p.info = pad256(((size_t)a.rows * a.n_kv * p.groups + 1) * 4);
+    if (a.n_prefix > 0) {
+      p.rows.prefix = true;
+      p.splits = p.rows.splits = rows_attn_splits(p.rows, a.n_prefix);
+      p.whole = pad256((size_t)a.rows * a.n_kv * p.groups * p.rc * row);
+    }
+  }
+  p.part = pad256((size_t)p.splits * a.n_kv * p.rows.R * row);
+  return p;
 }
 
 }  // namespace
 
-hipError_t launch_seq_attn(const SeqAttnArgs& a, hipStream_t s) {
-  if (a.rows == 0) return hipSuccess;
-  UAII_LAUNCH(k_seq_attn, dim3((unsigned)a.rows, (unsigned)a.n_heads), dim3(256), 0, s, a);
+size_t seq_attn_scratch(const SeqAttnArgs& a) { return plan_of(a).bytes(); }
+
+hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
+  Plan p = plan_of(a);
+  if (a.rows <= 0 || (p.bytes() > 0 && !scratch)) return hipErrorInvalidValue;
+  JoinArgs j{};
+  j.a = a;
+  j.G = p.G;
+  j.groups = j.rc = 1;
+  j.splits = p.splits;
+  j.part = p.rows.part = reinterpret_cast<float*>(scratch);
+  hipError_t e = hipSuccess;
+  if (!a.n_keys || p.splits > 0) {
+    e = launch_rows_attn(p.rows, s);
+    if (e != hipSuccess || (!a.n_keys && p.splits == 0)) return e;
+  }
+  if (a.n_keys) {
+    BatchArgs b{};
+    b.a = a;
+    b.G = p.G;
+    b.groups = p.groups;
+    b.slots = reinterpret_cast<float*>(scratch + p.part);
+    b.whole = reinterpret_cast<float*>(scratch + p.part + p.slots);
+    b.info = reinterpret_cast<int*>(scratch + p.part + p.slots + p.whole);
+    b.pre = j.part;
+    b.pre_splits = p.splits;
+    b.blocks = p.blocks;
+    switch (a.type) {
+      case KV_F32: e = by_width<KV_F32>(b, false, s); break;
+      case KV_F16: e = by_width<KV_F16>(b, p.pack, s); break;
+      case KV_Q8: e = by_width<KV_Q8>(b, p.pack, s); break;
+      default: return hipErrorInvalidValue;
+    }
+    if (e != hipSuccess) return e;
+    j.rc = p.rc;
+    j.groups = p.groups;
+    j.blocks = p.blocks;
+    j.slots = b.slots;
+    j.whole = b.whole;
+    j.info = b.info;
+  }
+  UAII_LAUNCH(k_attn_join, dim3((unsigned)(a.rows * a.n_heads)), dim3(256), 0, s, j);
   return hipGetLastError();
 }
 

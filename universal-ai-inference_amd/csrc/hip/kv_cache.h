@@ -65,6 +65,8 @@ struct SeqAttnArgs {
   const int32_t* first;
 };
 
-hipError_t launch_seq_attn(const SeqAttnArgs& a, hipStream_t s);
+// Device scratch of the call, and its launches.
+size_t seq_attn_scratch(const SeqAttnArgs& a);
+hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s);
 
 }  // namespace uaii_hip

@@ -1,0 +1,76 @@
+// seq_attn.h — what the attention kernels over the caches of a batch share.
+#pragma once
+
+#include "kv_cache.h"
+
+namespace uaii_hip {
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 h4_t __attribute__((ext_vector_type(4)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+typedef float f2_t __attribute__((ext_vector_type(2)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));  // rows of a caller's buffer start at any float
+typedef float f16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ inline float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
+
+// Power of two that brings the largest magnitude `top` of a row into [2^14, 2^15), as an
+// exponent: an f16 below 2^-14 would lose significant bits.
+__device__ inline int row_exponent(float top) {
+  if (!(top > 0.0f)) return 0;
+  return min(100, max(-113, 15 - ((int)((__float_as_uint(top) >> 23) & 0xff) - 126)));
+}
+
+// Two f32 as f16 pairs hi + lo, about 22 significant bits together.
+__device__ inline void split2(float a, float b, h2_t& hi, h2_t& lo) {
+  hi = __builtin_convertvector((f2_t{a, b}), h2_t);
+  lo = __builtin_convertvector((f2_t{fmaf((float)hi.x, -1.0f, a), fmaf((float)hi.y, -1.0f, b)}), h2_t);
+}
+
+// The 8-bit values of a word, (byte - 128) 2^-9 in f16: the byte as an f16 subnormal
+// (byte 2^-24) times 2^15, less 2^-2, one fused operation a pair and exact.
+__device__ inline h2_t q8_pair(uint32_t bytes_0_and_2) {
+  const h2_t up = {(_Float16)32768.0f, (_Float16)32768.0f}, off = {(_Float16)-0.25f, (_Float16)-0.25f};
+  return __builtin_elementwise_fma(__builtin_bit_cast(h2_t, bytes_0_and_2), up, off);
+}
+constexpr float kQ8Unit = 512.0f;  // 2^9: what a product of such values is multiplied by
+
+// tanh to 2 units in the last place: near 0 a quotient of polynomials (the fifth
+// convergent of tanh's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + ...))), which is
+// off by less than 2^-25 up to 0.9), further out (1 - t) / (1 + t) with t = exp(-2 |x|).
+__device__ inline float tanh_near(float x) {
+  const float x2 = x * x;
+  const float n = fmaf(x2, x2 + 105.0f, 945.0f), d = fmaf(x2, fmaf(x2, 15.0f, 420.0f), 945.0f);
+  return x * n * __builtin_amdgcn_rcpf(d);
+}
+__device__ inline float tanh_far(float x) {
+  const float t = __builtin_amdgcn_exp2f(-2.0f * kLog2e * fabsf(x));
+  return copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
+}
+
+// Attention partials of a row: [hd] sums of p v, then the running maximum (base 2) and
+// sum of p; 4 floats for those two keep rows 16-byte aligned.
+__host__ __device__ inline int64_t part_stride(int hd) { return hd + 4; }
+
+// ---- rows_attn.hip: many rows over one cache -------------------------------------------
+
+// Rows of one kv head are its G query heads' rows of query 0, of query 1, and so on:
+// row r is query r / G, head r % G. The keys are positions of one cache (kc, vc of `a`,
+// or its prefix).
+struct RowsAttnArgs {
+  SeqAttnArgs a;
+  int64_t R;      // rows of a kv head
+  int G, splits;  // key splits; with more than one, and for a prefix, partials are written
+  bool prefix;    // keys 0 .. n_prefix - 1 of kp, vp, for one query a sequence
+  float* part;    // [splits][n_kv][R][part_stride]
+};
+
+// Key splits that fill the device (1: none needed).
+int rows_attn_splits(const RowsAttnArgs& r, int64_t keys);
+hipError_t launch_rows_attn(const RowsAttnArgs& r, hipStream_t s);
+
+}  // namespace uaii_hip

@@ -4,6 +4,7 @@
 #include "uaii_hip.h"
 
 #include "hip/kv_cache.h"
+#include "scratch.h"
 
 #include <cmath>
 #include <cstdint>
@@ -13,12 +14,13 @@ using namespace uaii_hip;
 namespace {
 
 constexpr int kErrArg = -1;  // invalid argument
+constexpr int64_t kMaxPositions = (int64_t)1 << 30;  // positions and steps past them are 32-bit in the kernels
 
 hipStream_t S(void* s) { return static_cast<hipStream_t>(s); }
 
 bool layout_ok(int kv_type, int n_kv_heads, int head_dim, int64_t max_seq) {
   return (kv_type == KV_F32 || kv_type == KV_F16 || kv_type == KV_Q8) && n_kv_heads > 0 && n_kv_heads <= 65535 &&
-         head_dim >= 16 && head_dim <= 256 && head_dim % 16 == 0 && max_seq > 0 && max_seq <= INT32_MAX;
+         head_dim >= 16 && head_dim <= 256 && head_dim % 16 == 0 && max_seq > 0 && max_seq <= kMaxPositions;
 }
 
 bool aligned16(const void* p) { return p && (uintptr_t)p % 16 == 0; }
@@ -94,6 +96,16 @@ bool attn_args(const float* q, int64_t ldq, int64_t rows, const void* kcache, co
   return true;
 }
 
+int attend(const SeqAttnArgs& a, void* stream) {
+  uaii::Scratch scratch(S(stream));
+  const size_t bytes = seq_attn_scratch(a);
+  if (bytes > 0) {
+    const hipError_t e = scratch.reserve(bytes);
+    if (e != hipSuccess) return (int)e;
+  }
+  return (int)launch_seq_attn(a, scratch.data(), S(stream));
+}
+
 }  // namespace
 
 extern "C" {
@@ -140,8 +152,8 @@ int uaii_hip_attention_batch(const float* q, int64_t ldq, int64_t n_seq, const v
   SeqAttnArgs a{};
   if (!attn_args(q, ldq, n_seq, kcache, vcache, kv_type, max_seq, n_heads, n_kv_heads, head_dim, options, out, ldo, &a))
     return kErrArg;
-  if (n_prefix < 0 || n_prefix > INT32_MAX - max_seq) return kErrArg;  // positions are 32-bit in the kernels
-  if (n_prefix > 0 && (!aligned16(kprefix) || !aligned16(vprefix) || prefix_seq < n_prefix || prefix_seq > INT32_MAX))
+  if (n_prefix < 0 || n_prefix > kMaxPositions - max_seq) return kErrArg;
+  if (n_prefix > 0 && (!aligned16(kprefix) || !aligned16(vprefix) || prefix_seq < n_prefix || prefix_seq > kMaxPositions))
     return kErrArg;
   if (n_seq == 0) return 0;
   if (!aligned4(n_keys)) return kErrArg;
@@ -150,7 +162,7 @@ int uaii_hip_attention_batch(const float* q, int64_t ldq, int64_t n_seq, const v
   a.vp = static_cast<const uint8_t*>(vprefix);
   a.pre_seq = prefix_seq;
   a.n_prefix = (int)n_prefix;
-  return (int)launch_seq_attn(a, S(stream));
+  return attend(a, stream);
 }
 
 int uaii_hip_attention_prompt(const float* q, int64_t ldq, int64_t m, const void* kcache, const void* vcache,
@@ -167,7 +179,7 @@ int uaii_hip_attention_prompt(const float* q, int64_t ldq, int64_t m, const void
   a.p0 = (int)p0;
   a.bidir = (int)bidirectional;
   a.first = first_key;
-  return (int)launch_seq_attn(a, S(stream));
+  return attend(a, stream);
 }
 
 }  // extern "C"
