@@ -10,6 +10,7 @@
 #include "seq_attn.h"
 
 #include <algorithm>
+#include <atomic>
 
 namespace uaii_hip {
 namespace {
@@ -29,12 +30,6 @@ struct BatchArgs {
 __device__ inline f4_t mfma32(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ inline f4_t mfma16(h4_t a, h4_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
 __device__ inline f4_t mfma4(float a, float b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
-
-// Weight of a partial with running maximum m and sum l; a sum that is NaN stays in.
-__device__ inline float weight_of(float m, float l, float M) {
-  if (l != l) return 1.0f;
-  return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-}
 
 struct Span {
   int n, lo;  // keys lo .. n - 1 of the sequence
@@ -70,10 +65,10 @@ __device__ inline void load_words(const uint8_t* p, uint32_t (&w)[N]) {
 constexpr int rows_of(bool pack) { return pack ? 8 : 16; }
 
 template <int TYPE, int HD, bool PACK>
-__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs b) {
+__global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 1 : 2) k_batch_attn(BatchArgs b) {
   constexpr int NW = 4;
   constexpr int ES = TYPE == KV_F32 ? 4 : TYPE == KV_F16 ? 2 : 1;
-  constexpr int NS = TYPE == KV_F32 || (TYPE == KV_F16 && HD == 256) ? 1 : 2;  // 16-key subtiles of a tile
+  constexpr int NS = TYPE == KV_F32 || HD == 256 ? 1 : 2;  // 16-key subtiles of a tile
   constexpr int KT = 16 * NS;
   constexpr int RC = rows_of(PACK);
   constexpr int E = HD / 16;                // value dims of a lane
@@ -164,75 +159,80 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs
     kbase += first * a.hd * ES;
     vbase += first * a.hd * ES;
 
-    struct Tile {
-      uint32_t k[NS][KW], v[NS][4][VW];
-      float f;
-    } t0, t1;
+    uint32_t kw[NS][KW], vw[NS][4][VW];  // a tile: the lane's parts of its keys and of its values
+    float fw;                            // KV_Q8: a key's factor in the lower lanes, a value's in the upper
     // keys behind the last repeat it and are masked; dims behind the row's end repeat its
     // last piece, which meets zeros of q or goes to outputs that are not stored
-    auto load = [&](int t, Tile& x) __attribute__((always_inline)) {
+    const uint32_t row_bytes = (uint32_t)a.hd * ES;
+    auto load_keys = [&](int t) __attribute__((always_inline)) {
+      const uint8_t* kt = uniform_at(kbase, (int64_t)t * row_bytes);
+      const int last = __builtin_amdgcn_readfirstlane(k1 - 1 - t);
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        const uint8_t* kr = kbase + (int64_t)min(t + 16 * i + col, k1 - 1) * a.hd * ES;
+        const uint32_t kr = (uint32_t)min(16 * i + col, last) * row_bytes;
 #pragma unroll
         for (int w = 0; w < KW; w += 4) {
           constexpr int P = 16 / ES;
-          const int d = min(g * (HD / 4) + w / 4 * P, a.hd - P);
-          const u4_t y = *reinterpret_cast<const u4_t*>(kr + d * ES);
-          x.k[i][w] = y[0], x.k[i][w + 1] = y[1], x.k[i][w + 2] = y[2], x.k[i][w + 3] = y[3];
+          const u4_t y = *reinterpret_cast<const u4_t*>(kt + (kr + (uint32_t)min(g * (HD / 4) + w / 4 * P, a.hd - P) * ES));
+          kw[i][w] = y[0], kw[i][w + 1] = y[1], kw[i][w + 2] = y[2], kw[i][w + 3] = y[3];
         }
       }
-      const int d = min(col * E, a.hd - E);
+      if constexpr (SC) fw = (lane < 32 ? kscale : vscale)[t + min(lane & 31, last)];
+    };
+    auto load_values = [&](int t) __attribute__((always_inline)) {
+      const uint8_t* vt = uniform_at(vbase, (int64_t)t * row_bytes);
+      const int last = __builtin_amdgcn_readfirstlane(k1 - 1 - t);
+      const uint32_t d = (uint32_t)min(col * E, a.hd - E) * ES;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          load_words<VW>(vbase + ((int64_t)min(t + 16 * i + 4 * g + r, k1 - 1) * a.hd + d) * ES, x.v[i][r]);
-      if constexpr (SC) x.f = (lane < 32 ? kscale : vscale)[min(t + (lane & 31), k1 - 1)];
+        for (int r = 0; r < 4; ++r) load_words<VW>(vt + ((uint32_t)min(16 * i + 4 * g + r, last) * row_bytes + d), vw[i][r]);
     };
 
-    const int step = NW * KT, mine = k0 + wave * KT;
-    if (mine < k1) load(mine, t0);
-
-    // ---- q into fragments in LDS
-    const float* qrow = a.q + (int64_t)s * a.ldq + (int64_t)head0 * a.hd;
-    if constexpr (TYPE != KV_F32) {
-      // 16 lanes a row: its largest magnitude, for the power of two that it is scaled by
-      const int r = tid >> 4;
-      float top = 0.0f;
-      if (r < rows)
-        for (int d = tid & 15; d < a.hd; d += 16) top = fmaxf(top, fabsf(qrow[(int64_t)r * a.hd + d] * a.scale));
+    // q's part of a thread (row tid / 16, E dims), ahead of the first tile, so that nothing
+    // waits for the tile with it
+    const int qr = tid >> 4, qd = (tid & 15) * E;
+    float qv[E];
+    if (qr < rows) {
+      const float* at = a.q + (int64_t)s * a.ldq + (int64_t)(head0 + qr) * a.hd + min(qd, a.hd - E);
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-      if ((tid & 15) == 0) qtop[r] = top;
-      __syncthreads();
-      for (int x = tid; x < NC * 64; x += 256) {
-        const int c = x >> 6, ln = x & 63, cc = ln & 15, d0 = (ln >> 4) * (HD / 4) + 8 * c, rr = PACK ? cc & 7 : cc;
-        const float up = pow2i(row_exponent(qtop[rr]));
-        h8_t hi, lo;
-#pragma unroll
-        for (int k = 0; k < 8; k += 2) {
-          // bytes of a word pair up as 0 and 2, 1 and 3
-          const int ka = TYPE == KV_Q8 ? (k & 4) + (k >> 1 & 1) : k, kb = TYPE == KV_Q8 ? ka + 2 : k + 1;
-          const bool in = rr < rows && d0 < a.hd;
-          const float va = in ? qrow[(int64_t)rr * a.hd + d0 + ka] * a.scale * up : 0.0f;
-          const float vb = in ? qrow[(int64_t)rr * a.hd + d0 + kb] * a.scale * up : 0.0f;
-          h2_t p, q;
-          split2(va, vb, p, q);
-          hi[k] = p.x, hi[k + 1] = p.y, lo[k] = q.x, lo[k + 1] = q.y;
-        }
-        h8_t* to = reinterpret_cast<h8_t*>(qf);
-        if constexpr (PACK) {
-          to[x] = cc >= 8 ? lo : hi;
-        } else {
-          to[x] = hi;
-          to[NC * 64 + x] = lo;
-        }
+      for (int e = 0; e < E; e += 4) {
+        const f4_t x = *reinterpret_cast<const f4u_t*>(at + e);
+        qv[e] = x[0], qv[e + 1] = x[1], qv[e + 2] = x[2], qv[e + 3] = x[3];
       }
-    } else {
-      for (int x = tid; x < HD / 4 * 64; x += 256) {
-        const int ln = x >> 2 & 63, d = (ln >> 4) * (HD / 4) + (x >> 8) * 4 + (x & 3), rr = ln & 15;
-        qf[x] = __float_as_uint(rr < rows && d < a.hd ? qrow[(int64_t)rr * a.hd + d] * a.scale : 0.0f);
+    }
+    const int step = NW * KT, mine = k0 + wave * KT;
+    if (mine < k1) load_keys(mine), load_values(mine);
+
+    // ---- q as fragments in LDS, f16 halves scaled to the row's largest magnitude
+    {
+      float top = 0.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        qv[e] = qr < rows && qd < a.hd ? qv[e] * a.scale : 0.0f;
+        top = fmaxf(top, fabsf(qv[e]));
+      }
+#pragma unroll
+      for (int k = 8; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
+      if ((tid & 15) == 0) qtop[qr] = top;
+      const float up = TYPE == KV_F32 ? 1.0f : pow2i(row_exponent(top));
+      if (qr < RC) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+          const int d = qd + e, part = d / (HD / 4), at = d % (HD / 4);  // lanes 16 part .. + 15 hold it
+          if constexpr (TYPE == KV_F32) {
+            reinterpret_cast<f4_t*>(qf)[at / 4 * 64 + 16 * part + qr] = f4_t{qv[e], qv[e + 1], qv[e + 2], qv[e + 3]};
+          } else {
+            // bytes of a word pair up as 0 and 2, 1 and 3
+            constexpr int B = TYPE == KV_Q8 ? 2 : 1, C = TYPE == KV_Q8 ? 1 : 2;
+            h2_t h0, h1, l0, l1;
+            split2(qv[e] * up, qv[e + B] * up, h0, l0);
+            split2(qv[e + C] * up, qv[e + 3] * up, h1, l1);
+            h4_t* to = reinterpret_cast<h4_t*>(qf) + (at / 8 * 64 + 16 * part + qr) * 2 + at / 4 % 2;
+            to[0] = h4_t{h0.x, h0.y, h1.x, h1.y};
+            to[PACK ? 16 : NC * 128] = h4_t{l0.x, l0.y, l1.x, l1.y};
+          }
+        }
       }
     }
     __syncthreads();
@@ -247,11 +247,14 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs
     // as in rows_attn.hip: probabilities are 2^(y - m + 10) / D
     float m = -INFINITY, l = 0.0f, D = SC ? 0x1p-60f : 1.0f, lgD = SC ? -60.0f : 0.0f;
 
-    auto tile = [&](int t, const Tile& x) __attribute__((always_inline)) {
+    // A tile's keys are used up before its softmax and its values behind it: the next tile's
+    // are loaded into the same registers from there on, and are on their way through the other
+    // half of the work.
+    for (int t = mine; t < k1; t += step) {
       f4_t y[NS];
       if constexpr (SC) {
-        sc[wave][lane] = x.f;
-        const float f = lane >= 32 ? x.f : 0.0f;
+        sc[wave][lane] = fw;
+        const float f = lane >= 32 ? fw : 0.0f;
         if (__any(f > D && f < INFINITY)) {
           const float top = wave_max_dpp(f < INFINITY ? f : 0.0f);
           const int e = min(126, (int)((__float_as_uint(top) >> 23) & 0xff) - 126);
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs
         for (int w = 0; w < KW; w += 4) {
           const f4_t q = reinterpret_cast<const f4_t*>(qf)[w / 4 * 64 + lane];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) y[0] = mfma4(__uint_as_float(x.k[0][w + k]), q[k], y[0]);
+          for (int k = 0; k < 4; ++k) y[0] = mfma4(__uint_as_float(kw[0][w + k]), q[k], y[0]);
         }
       } else {
 #pragma unroll
@@ -282,11 +285,11 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs
           for (int i = 0; i < NS; ++i) {
             h8_t kf;
             if constexpr (TYPE == KV_F16) {
-              kf = __builtin_bit_cast(h8_t, (u4_t{x.k[i][4 * c], x.k[i][4 * c + 1], x.k[i][4 * c + 2], x.k[i][4 * c + 3]}));
+              kf = __builtin_bit_cast(h8_t, (u4_t{kw[i][4 * c], kw[i][4 * c + 1], kw[i][4 * c + 2], kw[i][4 * c + 3]}));
             } else {
 #pragma unroll
               for (int w = 0; w < 2; ++w) {
-                const uint32_t z = x.k[i][2 * c + w];
+                const uint32_t z = kw[i][2 * c + w];
                 const h2_t p = q8_pair(z & 0x00ff00ffu), q = q8_pair(__builtin_amdgcn_perm(0, z, 0x0c030c01));
                 kf[4 * w] = p.x, kf[4 * w + 1] = p.y, kf[4 * w + 2] = q.x, kf[4 * w + 3] = q.y;
               }
@@ -302,6 +305,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs
             for (int r = 0; r < 4; ++r) y[i][r] += dpp_mov<0x128>(y[i][r]);  // row_ror 8: the other half's column
         }
       }
+      const int next = t + step < k1 ? t + step : t;  // the last turn loads its own tile again
+      load_keys(next);
       // element r of y[i]: key t + 16 i + 4 g + r
       f4_t vf[NS];
       if constexpr (SC) {
@@ -323,14 +328,13 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs
             y[i][r] *= to_cap;
             far = fmaxf(far, fabsf(y[i][r]));
           }
-        const bool some_far = __any(!(far < 0.9f));
+        const bool some_far = __any(!(far < kTanhNear));
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float z = y[i][r];
-            y[i][r] = tanh_near(z);
-            if (some_far) y[i][r] = fabsf(z) < 0.9f ? y[i][r] : tanh_far(z);
+            const float near = tanh_near(y[i][r]);
+            y[i][r] = some_far && !(fabsf(y[i][r]) < kTanhNear) ? tanh_far(y[i][r]) : near;
           }
       }
       if (sloped) {
@@ -380,7 +384,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[e] = mfma4(__uint_as_float(x.v[0][r][e]), y[0][r], o[e]);
+          for (int e = 0; e < E; ++e) o[e] = mfma4(__uint_as_float(vw[0][r][e]), y[0][r], o[e]);
       } else {
         h4_t p0[NS], p1[NS];
 #pragma unroll
@@ -405,9 +409,9 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs
             for (int r = 0; r < 4; r += 2) {
               h2_t z;
               if constexpr (TYPE == KV_F16) {
-                z = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(x.v[i][r + 1][e / 2], x.v[i][r][e / 2], e & 1 ? 0x07060302 : 0x05040100));
+                z = __builtin_bit_cast(h2_t, __builtin_amdgcn_perm(vw[i][r + 1][e / 2], vw[i][r][e / 2], e & 1 ? 0x07060302 : 0x05040100));
               } else {
-                z = q8_pair(__builtin_amdgcn_perm(x.v[i][r + 1][e / 4], x.v[i][r][e / 4], 0x0c040c00 + (e & 3) * 0x00010001));
+                z = q8_pair(__builtin_amdgcn_perm(vw[i][r + 1][e / 4], vw[i][r][e / 4], 0x0c040c00 + (e & 3) * 0x00010001));
               }
               vv[i][r] = z.x, vv[i][r + 1] = z.y;
             }
@@ -421,14 +425,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs
           }
         }
       }
-    };
-
-    for (int t = mine; t < k1; t += 2 * step) {
-      if (t + step < k1) load(t + step, t1);
-      tile(t, t0);
-      if (t + step >= k1) break;
-      if (t + 2 * step < k1) load(t + 2 * step, t0);
-      tile(t + step, t1);
+      load_values(next);
     }
 
     // ---- the waves' results together
@@ -484,8 +481,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_batch_attn(BatchArgs
   }
 }
 
-// Partial results of a row into its output: block (row, query head), the waves taking
-// partials in turn.
+// Partial results of a row into its output: a block of W waves for each (row, query head),
+// eight partials of a wave at a time.
 struct JoinArgs {
   SeqAttnArgs a;
   int G, rc, groups, blocks;
@@ -496,12 +493,13 @@ struct JoinArgs {
   int splits;
 };
 
-__global__ void __launch_bounds__(256) k_attn_join(JoinArgs j) {
-  __shared__ float wm[4], wl[4];
-  __shared__ __attribute__((aligned(16))) float wo[4][256];
+template <int W>
+__global__ void __launch_bounds__(64 * W) k_attn_join(JoinArgs j) {
+  __shared__ float wm[W], wl[W];
+  __shared__ __attribute__((aligned(16))) float wo[W][256];
   const SeqAttnArgs& a = j.a;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int row = (int)(blockIdx.x / (unsigned)a.n_heads), head = (int)(blockIdx.x % (unsigned)a.n_heads);
   const int kvh = head / j.G, gr = head % j.G, H = a.n_kv * j.groups;
   const int64_t stride = part_stride(a.hd);
@@ -532,24 +530,25 @@ __global__ void __launch_bounds__(256) k_attn_join(JoinArgs j) {
   const int n = own + j.splits, d = min(4 * lane, a.hd - 4);
   float m = -INFINITY, l = 0.0f;
   f4_t o = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int i0 = wave; i0 < n; i0 += 16) {
-    float mi[4], li[4];
-    f4_t oi[4];
+  constexpr int U = 8;
+  for (int i0 = wave; i0 < n; i0 += U * W) {
+    float mi[U], li[U];
+    f4_t oi[U];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float* p = part_of(min(i0 + 4 * k, n - 1));
+    for (int k = 0; k < U; ++k) {
+      const float* p = part_of(min(i0 + k * W, n - 1));
       mi[k] = p[a.hd], li[k] = p[a.hd + 1];
       oi[k] = *reinterpret_cast<const f4_t*>(p + d);
     }
     float M = m;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) M = i0 + 4 * k < n ? fmaxf(M, mi[k]) : M;
+    for (int k = 0; k < U; ++k) M = i0 + k * W < n ? fmaxf(M, mi[k]) : M;
     const float keep = weight_of(m, l, M);
     l *= keep;
     o *= keep;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (i0 + 4 * k >= n) continue;
+    for (int k = 0; k < U; ++k) {
+      if (i0 + k * W >= n) continue;
       const float f = weight_of(mi[k], li[k], M);
       l += f * li[k];
       o += f * oi[k];
@@ -562,10 +561,10 @@ __global__ void __launch_bounds__(256) k_attn_join(JoinArgs j) {
   if (wave != 0 || 4 * lane >= a.hd) return;
   float M = -INFINITY, den = 0.0f;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, wm[w]);
+  for (int w = 0; w < W; ++w) M = fmaxf(M, wm[w]);
   f4_t acc = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
+  for (int w = 0; w < W; ++w) {
     const float f = weight_of(wm[w], wl[w], M);
     den += f * wl[w];
     acc += f * *reinterpret_cast<const f4_t*>(&wo[w][4 * lane]);
@@ -574,24 +573,36 @@ __global__ void __launch_bounds__(256) k_attn_join(JoinArgs j) {
   *reinterpret_cast<f4u_t*>(a.out + (int64_t)row * a.ldo + (int64_t)head * a.hd + 4 * lane) = acc * inv;
 }
 
-template <int TYPE, int HD, bool PACK>
-hipError_t go(BatchArgs& b, hipStream_t s) {
-  UAII_LAUNCH((k_batch_attn<TYPE, HD, PACK>), dim3((unsigned)b.blocks), dim3(256), 0, s, b);
-  return hipGetLastError();
+// Calls f with the kernel of the call's type, width and row packing.
+template <typename F>
+auto with_kernel(int type, int hd, bool pack, F f) {
+  const int w = hd <= 64 ? 0 : hd <= 128 ? 1 : 2;
+  if (type == KV_F32) return w == 0 ? f(&k_batch_attn<KV_F32, 64, false>) : w == 1 ? f(&k_batch_attn<KV_F32, 128, false>) : f(&k_batch_attn<KV_F32, 256, false>);
+  if (type == KV_F16) {
+    if (pack) return w == 0 ? f(&k_batch_attn<KV_F16, 64, true>) : w == 1 ? f(&k_batch_attn<KV_F16, 128, true>) : f(&k_batch_attn<KV_F16, 256, true>);
+    return w == 0 ? f(&k_batch_attn<KV_F16, 64, false>) : w == 1 ? f(&k_batch_attn<KV_F16, 128, false>) : f(&k_batch_attn<KV_F16, 256, false>);
+  }
+  if (pack) return w == 0 ? f(&k_batch_attn<KV_Q8, 64, true>) : w == 1 ? f(&k_batch_attn<KV_Q8, 128, true>) : f(&k_batch_attn<KV_Q8, 256, true>);
+  return w == 0 ? f(&k_batch_attn<KV_Q8, 64, false>) : w == 1 ? f(&k_batch_attn<KV_Q8, 128, false>) : f(&k_batch_attn<KV_Q8, 256, false>);
 }
 
-template <int TYPE>
-hipError_t by_width(BatchArgs& b, bool pack, hipStream_t s) {
-  if constexpr (TYPE != KV_F32) {
-    if (pack) {
-      if (b.a.hd <= 64) return go<TYPE, 64, true>(b, s);
-      if (b.a.hd <= 128) return go<TYPE, 128, true>(b, s);
-      return go<TYPE, 256, true>(b, s);
-    }
+// Blocks of that kernel that the device holds at once (asked once for each).
+int resident_blocks(int type, int hd, bool pack) {
+  static std::atomic<int> known[3][3][2];
+  std::atomic<int>& k = known[type][hd <= 64 ? 0 : hd <= 128 ? 1 : 2][pack];
+  int n = k.load(std::memory_order_relaxed);
+  if (n == 0) {
+    n = with_kernel(type, hd, pack, [](auto kernel) {
+      int per_cu = 0;
+      if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kernel, 256, 0) != hipSuccess || per_cu < 1) {
+        (void)hipGetLastError();
+        per_cu = 1;
+      }
+      return per_cu;
+    }) * device_cus();
+    k.store(n, std::memory_order_relaxed);
   }
-  if (b.a.hd <= 64) return go<TYPE, 64, false>(b, s);
-  if (b.a.hd <= 128) return go<TYPE, 128, false>(b, s);
-  return go<TYPE, 256, false>(b, s);
+  return n;
 }
 
 struct Plan {
@@ -619,7 +630,7 @@ Plan plan_of(const SeqAttnArgs& a) {
     p.rc = rows_of(p.pack);
     p.groups = (p.G + p.rc - 1) / p.rc;
     const int64_t units = a.rows * a.n_kv * p.groups * ((a.max_seq + UNIT - 1) / UNIT);
-    p.blocks = (int)std::min<int64_t>(units, (int64_t)device_cus() * 2);
+    p.blocks = (int)std::min<int64_t>(units, resident_blocks(a.type, a.hd, p.pack));
     p.slots = pad256(2 * (size_t)p.blocks * p.rc * row);
     p.info = pad256(((size_t)a.rows * a.n_kv * p.groups + 1) * 4);
     if (a.n_prefix > 0) {
@@ -661,12 +672,10 @@ hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
     b.pre = j.part;
     b.pre_splits = p.splits;
     b.blocks = p.blocks;
-    switch (a.type) {
-      case KV_F32: e = by_width<KV_F32>(b, false, s); break;
-      case KV_F16: e = by_width<KV_F16>(b, p.pack, s); break;
-      case KV_Q8: e = by_width<KV_Q8>(b, p.pack, s); break;
-      default: return hipErrorInvalidValue;
-    }
+    e = with_kernel(a.type, a.hd, p.pack, [&](auto kernel) {
+      UAII_LAUNCH(kernel, dim3((unsigned)b.blocks), dim3(256), 0, s, b);
+      return hipGetLastError();
+    });
     if (e != hipSuccess) return e;
     j.rc = p.rc;
     j.groups = p.groups;
@@ -675,7 +684,12 @@ hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
     j.whole = b.whole;
     j.info = b.info;
   }
-  UAII_LAUNCH(k_attn_join, dim3((unsigned)(a.rows * a.n_heads)), dim3(256), 0, s, j);
+  // about how many partials a row has: a wave takes eight in one round trip
+  const int64_t parts = p.splits + (a.n_keys ? std::max<int64_t>(1, p.blocks / (a.rows * a.n_kv * p.groups)) : 0);
+  const dim3 grid((unsigned)(a.rows * a.n_heads));
+  if (parts <= 8) UAII_LAUNCH(k_attn_join<1>, grid, dim3(64), 0, s, j);
+  else if (parts <= 32) UAII_LAUNCH(k_attn_join<4>, grid, dim3(256), 0, s, j);
+  else UAII_LAUNCH(k_attn_join<16>, grid, dim3(1024), 0, s, j);
   return hipGetLastError();
 }
 

@@ -32,37 +32,62 @@ __device__ inline int wave_max_i(int v) {
   return v;
 }
 
-template <int TYPE, int NW>
+// A block has 4 waves: NR of them take 32 rows each, and the NK = 4 / NR groups of such waves
+// take the tiles of the block's keys in turn, each in an LDS region of its own.
+template <int TYPE, int NR>
 constexpr int tile_keys() {
-  return TYPE == KV_F32 || NW < 4 ? 32 : 64;
+  return TYPE == KV_F32 || NR < 4 ? 32 : 64;
 }
 
-template <int TYPE, int HD, int NW>
-__global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnArgs r) {
-  constexpr int NT = 64 * NW, TK = tile_keys<TYPE, NW>();
+// Whether the next 32 keys' products are started beside the softmax of the last: where the
+// registers hold them.
+#ifndef UAII_AHEAD
+#define UAII_AHEAD 0
+#endif
+template <int HD>
+constexpr bool ahead() { return HD != 128 || UAII_AHEAD; }
+
+template <int TYPE, int HD, int NR>
+__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnArgs r) {
+  constexpr int NK = 4 / NR, NT = 64 * NR, TK = tile_keys<TYPE, NR>(), SUBS = TK / 32;
+  constexpr int NB = NR == 1 ? 1 : 2;                   // buffers of a region; a lone wave needs one
+  constexpr bool QL = NR == 1;                          // q's fragments in LDS: the waves share their rows
   constexpr int PL = TYPE == KV_F32 ? 2 : 1;            // f16 planes of a tile (hi, lo)
   constexpr bool SC = TYPE != KV_F16;                   // a factor for each key
-  constexpr int KP = HD + 8;                            // tile row (halfs)
+  constexpr int KP = HD + 8, VP = HD + 16;              // rows of a tile (halfs): see v_at
   constexpr int NC = HD / 16, ND = HD / 32;             // dim chunks of S, dim tiles of O
   constexpr int PE = TYPE == KV_Q8 ? 16 : 8;            // dims of a staged piece
   constexpr int PR = HD / PE;                           // pieces of a key's row
   constexpr int PIECES = TK * PR / NT;
   constexpr int PW = TYPE == KV_F32 ? 2 : 1;            // 16-byte words of a piece
-  __shared__ __attribute__((aligned(16))) _Float16 ks[2][PL][TK * KP];
-  __shared__ __attribute__((aligned(16))) _Float16 vs[2][PL][TK * KP];
-  __shared__ __attribute__((aligned(16))) float ksc[2][SC ? TK : 4], vsc[2][SC ? TK : 4];
-  // non-finite values of a tile: a bit a dim, and whether a wave's pieces have one
-  __shared__ uint8_t nonfinite[2][SC && PL == 1 ? 1 : TK][HD / 8];
-  __shared__ int bad[2][NW], rng[NW][4];
+  struct Tile {
+    __attribute__((aligned(16))) _Float16 k[PL][TK * KP];
+    __attribute__((aligned(16))) _Float16 v[PL][TK * VP];
+    __attribute__((aligned(16))) float kf[SC ? TK : 4], vf[SC ? TK : 4];
+    // values that are not finite: a bit a dim (KV_Q8: one for the row), and whether a wave's
+    // pieces have one (KV_Q8: whether the tile has)
+    uint8_t marks[TK][TYPE == KV_Q8 ? 1 : HD / 8];
+    int bad[TYPE == KV_Q8 ? 1 : NR];
+  };
+  struct Merge {  // of the groups behind the first
+    f4_t o[NK > 1 ? NK - 1 : 1][NR][HD / 8][64];
+    float ml[NK > 1 ? NK - 1 : 1][NR][2][64], D[NK > 1 ? NK - 1 : 1][NR];
+  };
+  constexpr size_t kTiles = sizeof(Tile) * NB * NK, kMerge = NK > 1 ? sizeof(Merge) : 0;
+  __shared__ __attribute__((aligned(16))) char lds[kTiles > kMerge ? kTiles : kMerge];
+  __shared__ __attribute__((aligned(16))) h8_t qs[QL ? 2 * NC * 64 : 1];
+  __shared__ int rng[NR][4];
 
   const SeqAttnArgs& a = r.a;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = wave % NR, kg = wave / NR, tid = threadIdx.x - NT * kg;
   const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+  Tile* tiles = reinterpret_cast<Tile*>(lds) + NB * kg;
   const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv);
   const int sx = (int)(blockIdx.x / (unsigned)a.n_kv);
   const int split = sx % r.splits;
-  const int nx = (int)((r.R + 32 * NW - 1) / (32 * NW));
-  const int64_t row_at = (int64_t)(nx - 1 - sx / r.splits) * (32 * NW) + 32 * wave + col;  // the longest first
+  const int nx = (int)((r.R + 32 * NR - 1) / (32 * NR));
+  const int64_t row_at = (int64_t)(nx - 1 - sx / r.splits) * (32 * NR) + 32 * rw + col;  // the longest first
   const bool valid = row_at < r.R;
   const int64_t row = valid ? row_at : r.R - 1;
   const int query = (int)(row / r.G), head = kvh * r.G + (int)(row % r.G);
@@ -82,61 +107,21 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) k_rows_attn(RowsAt
   if (lo >= hi) lo = INT32_MAX, hi = 0;
   const int wlo = wave_min_i(lo), wlo_max = wave_max_i(lo), whi_min = wave_min_i(hi), whi = wave_max_i(hi);
   int blo = wlo, bhi = whi, blo_max = wlo_max, bhi_min = whi_min;
-  if constexpr (NW > 1) {
-    if (lane == 0) rng[wave][0] = wlo, rng[wave][1] = wlo_max, rng[wave][2] = whi_min, rng[wave][3] = whi;
+  if constexpr (NR > 1) {
+    if (lane == 0 && kg == 0) rng[rw][0] = wlo, rng[rw][1] = wlo_max, rng[rw][2] = whi_min, rng[rw][3] = whi;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
+    for (int w = 0; w < NR; ++w) {
       blo = min(blo, rng[w][0]), blo_max = max(blo_max, rng[w][1]);
       bhi_min = min(bhi_min, rng[w][2]), bhi = max(bhi, rng[w][3]);
     }
   }
   blo = __builtin_amdgcn_readfirstlane(blo), bhi = __builtin_amdgcn_readfirstlane(bhi);
+  if (blo >= bhi) blo = bhi = 0;  // no row sees a key: no tiles, and none behind the end of int for a later group
   // this split's tiles
-  const int tiles = bhi > blo ? (bhi - blo + TK - 1) / TK : 0;
-  const int tile0 = (int)((int64_t)tiles * split / r.splits), tile1 = (int)((int64_t)tiles * (split + 1) / r.splits);
+  const int n_tiles = (bhi - blo + TK - 1) / TK;
+  const int tile0 = (int)((int64_t)n_tiles * split / r.splits), tile1 = (int)((int64_t)n_tiles * (split + 1) / r.splits);
   const int k0 = blo + tile0 * TK, k1 = min(bhi, blo + tile1 * TK);
-
-  // q * scale * 2^e as f16 hi + lo: the lane has dims 16 c + 8 h .. + 7 of its row
-  h8_t qhi[NC], qlo[NC];
-  float unit;  // of a raw product
-  {
-    const float* qp = a.q + (int64_t)query * a.ldq + (int64_t)head * a.hd;
-    float qv[NC][8], top = 0.0f;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int d = 16 * c + 8 * h;
-      const f4_t x0 = *reinterpret_cast<const f4u_t*>(qp + min(d, a.hd - 8)), x1 = *reinterpret_cast<const f4u_t*>(qp + min(d, a.hd - 8) + 4);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        qv[c][k] = d < a.hd ? (k < 4 ? x0[k] : x1[k - 4]) * a.scale : 0.0f;
-        top = fmaxf(top, fabsf(qv[c][k]));
-      }
-    }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const int e = row_exponent(top);
-    const float up = pow2i(e);
-    unit = pow2i(-e) * (TYPE == KV_Q8 ? kQ8Unit : 1.0f);
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-      for (int k = 0; k < 8; k += 2) {
-        h2_t x, y;
-        split2(qv[c][k] * up, qv[c][k + 1] * up, x, y);
-        qhi[c][k] = x.x, qhi[c][k + 1] = x.y, qlo[c][k] = y.x, qlo[c][k + 1] = y.y;
-      }
-  }
-  const bool capped = a.cap > 0.0f, sloped = a.slopes != nullptr;
-  const float to_cap = capped ? unit / a.cap : 0.0f;
-  const float mul = (capped ? a.cap : unit) * kLog2e;  // scores in base 2
-  const float slope = sloped ? a.slopes[head] * kLog2e : 0.0f;
-
-  // The lane's row: probabilities are 2^(y - m + 10) / D. m follows the maximum in steps (a
-  // score may pass it by 2^4), D is a power of two over the values' factors so far.
-  f16_t o[ND];
-#pragma unroll
-  for (int d = 0; d < ND; ++d) o[d] = f16_t{};
-  float m = -INFINITY, l = 0.0f, D = SC ? 0x1p-60f : 1.0f, lgD = SC ? -60.0f : 0.0f;
 
   const int64_t seq = r.prefix ? a.pre_seq : a.max_seq;
   const uint8_t* kbase = r.prefix ? a.kp : a.kc;
@@ -152,21 +137,86 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) k_rows_attn(RowsAt
   float screg = 0.0f;
   // keys behind the last one repeat it, dims behind the last piece that piece: both are in
   // the cache, and masked or met by zeros of q
+  const uint32_t row_bytes = (uint32_t)a.hd * ES;
+  // (`slot` hides tid from the loop: its few additions again each turn, not their results in
+  // registers that the products need)
   auto load_tile = [&](int t) __attribute__((always_inline)) {
+    int slot = tid;
+    asm volatile("" : "+v"(slot));
+    const uint8_t* kt = uniform_at(kbase, (int64_t)t * row_bytes);
+    const uint8_t* vt = uniform_at(vbase, (int64_t)t * row_bytes);
+    const int last = __builtin_amdgcn_readfirstlane(k1 - 1 - t);
 #pragma unroll
     for (int u = 0; u < PIECES; ++u) {
-      const int c = threadIdx.x + NT * u, key = min(t + c / PR, k1 - 1), d = min(c % PR * PE, a.hd - PE);
-      const int64_t off = ((int64_t)key * a.hd + d) * ES;
+      const int c = slot + NT * u;
+      const uint32_t off = (uint32_t)min(c / PR, last) * row_bytes + (uint32_t)min(c % PR * PE, a.hd - PE) * ES;
 #pragma unroll
       for (int w = 0; w < PW; ++w) {
-        kreg[u][w] = *reinterpret_cast<const u4_t*>(kbase + off + 16 * w);
-        vreg[u][w] = *reinterpret_cast<const u4_t*>(vbase + off + 16 * w);
+        kreg[u][w] = *reinterpret_cast<const u4_t*>(kt + off + 16 * w);
+        vreg[u][w] = *reinterpret_cast<const u4_t*>(vt + off + 16 * w);
       }
     }
     if constexpr (TYPE == KV_Q8) {
-      if ((int)threadIdx.x < 2 * TK) screg = ((int)threadIdx.x < TK ? kscale : vscale)[min(t + (int)threadIdx.x % TK, k1 - 1)];
+      if (slot < 2 * TK) screg = (slot < TK ? kscale : vscale)[t + min(slot % TK, last)];
     }
   };
+  const int mine = k0 + kg * TK;  // the group's first tile
+
+  // q * scale * 2^e as f16 hi + lo: the lane has dims 16 c + 8 h .. + 7 of its row
+  h8_t qhi[QL ? 1 : NC], qlo[QL ? 1 : NC];
+  float unit;  // of a raw product
+  {
+    const float* qp = a.q + (int64_t)query * a.ldq + (int64_t)head * a.hd;
+    float qv[NC][8], top = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const float* at = qp + min(16 * c + 8 * h, a.hd - 8);
+      const f4_t x0 = *reinterpret_cast<const f4u_t*>(at), x1 = *reinterpret_cast<const f4u_t*>(at + 4);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) qv[c][k] = k < 4 ? x0[k] : x1[k - 4];
+    }
+    // behind q, so that nothing waits for the tile with it
+    if (mine < k1) load_tile(mine);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        qv[c][k] = 16 * c + 8 * h < a.hd ? qv[c][k] * a.scale : 0.0f;
+        top = fmaxf(top, fabsf(qv[c][k]));
+      }
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const int e = row_exponent(top);
+    const float up = pow2i(e);
+    unit = pow2i(-e) * (TYPE == KV_Q8 ? kQ8Unit : 1.0f);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      h8_t hi8, lo8;
+#pragma unroll
+      for (int k = 0; k < 8; k += 2) {
+        h2_t x, y;
+        split2(qv[c][k] * up, qv[c][k + 1] * up, x, y);
+        hi8[k] = x.x, hi8[k + 1] = x.y, lo8[k] = y.x, lo8[k + 1] = y.y;
+      }
+      if constexpr (QL) {
+        if (c % NK == kg) qs[64 * c + lane] = hi8, qs[64 * (NC + c) + lane] = lo8;
+      } else {
+        qhi[c] = hi8, qlo[c] = lo8;
+      }
+    }
+    if constexpr (QL) __syncthreads();
+  }
+  const bool capped = a.cap > 0.0f, sloped = a.slopes != nullptr;
+  const float to_cap = capped ? unit / a.cap : 0.0f;
+  const float mul = (capped ? a.cap : unit) * kLog2e;  // scores in base 2
+  const float slope = sloped ? a.slopes[head] * kLog2e : 0.0f;
+
+  // The lane's row: probabilities are 2^(y - m + 10) / D. m follows the maximum in steps (a
+  // score may pass it by 2^4), D is a power of two over the values' factors so far.
+  f16_t o[ND];
+#pragma unroll
+  for (int d = 0; d < ND; ++d) o[d] = f16_t{};
+  float m = -INFINITY, l = 0.0f, D = SC ? 0x1p-60f : 1.0f, lgD = SC ? -60.0f : 0.0f;
+
   // f32 pieces: rows scaled to their largest finite magnitude, as hi + lo
   auto store_f32 = [&](const u4_t (&x)[PW], _Float16* hi_at, _Float16* lo_at, float* factor) __attribute__((always_inline)) {
     if constexpr (TYPE == KV_F32) {
@@ -193,7 +243,9 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) k_rows_attn(RowsAt
       if (factor) *factor = pow2i(-e);
     }
   };
-  auto store_tile = [&](int t, int buf) __attribute__((always_inline)) {
+  auto store_tile = [&](int t, Tile& to) __attribute__((always_inline)) {
+    int slot = tid;
+    asm volatile("" : "+v"(slot));
     // Where some row does not see some key, a probability of 0 must not meet a value that is
     // not finite: such values are stored as 0 and marked.
     if constexpr (TYPE != KV_Q8) {
@@ -211,7 +263,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) k_rows_attn(RowsAt
         if (any) {
 #pragma unroll
           for (int u = 0; u < PIECES; ++u) {
-            const int c = threadIdx.x + NT * u;
+            const int c = slot + NT * u;
             uint32_t bits = 0;
 #pragma unroll
             for (int w = 0; w < 4 * PW; ++w) {
@@ -227,18 +279,19 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) k_rows_attn(RowsAt
               }
               vreg[u][w / 4][w % 4] = x;
             }
-            nonfinite[buf][c / PR][c % PR] = (uint8_t)bits;
+            to.marks[c / PR][c % PR] = (uint8_t)bits;
           }
         }
       }
-      if (lane == 0) bad[buf][wave] = any;
+      if (lane == 0) to.bad[rw] = any;
     }
 #pragma unroll
     for (int u = 0; u < PIECES; ++u) {
-      const int c = threadIdx.x + NT * u, key = c / PR, at = key * KP + c % PR * PE;
+      const int c = slot + NT * u, key = c / PR, d = c % PR * PE;
+      _Float16 *kt = &to.k[0][key * KP + d], *vt = &to.v[0][key * VP + d];
       if constexpr (TYPE == KV_F16) {
-        *reinterpret_cast<u4_t*>(&ks[buf][0][at]) = kreg[u][0];
-        *reinterpret_cast<u4_t*>(&vs[buf][0][at]) = vreg[u][0];
+        *reinterpret_cast<u4_t*>(kt) = kreg[u][0];
+        *reinterpret_cast<u4_t*>(vt) = vreg[u][0];
       } else if constexpr (TYPE == KV_Q8) {
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
@@ -247,198 +300,243 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) k_rows_attn(RowsAt
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const h2_t p = q8_pair(__builtin_amdgcn_perm(0, x[w], 0x0c010c00)), q = q8_pair(__builtin_amdgcn_perm(0, x[w], 0x0c030c02));
-            h8_t& to = y[w / 2];
-            to[4 * (w % 2)] = p.x, to[4 * (w % 2) + 1] = p.y, to[4 * (w % 2) + 2] = q.x, to[4 * (w % 2) + 3] = q.y;
+            h8_t& z = y[w / 2];
+            z[4 * (w % 2)] = p.x, z[4 * (w % 2) + 1] = p.y, z[4 * (w % 2) + 2] = q.x, z[4 * (w % 2) + 3] = q.y;
           }
-          _Float16* to = kv ? &vs[buf][0][at] : &ks[buf][0][at];
-          *reinterpret_cast<h8_t*>(to) = y[0];
-          *reinterpret_cast<h8_t*>(to + 8) = y[1];
+          h8_t* at = reinterpret_cast<h8_t*>(kv ? vt : kt);
+          at[0] = y[0], at[1] = y[1];
         }
       } else {
-        store_f32(kreg[u], &ks[buf][0][at], &ks[buf][PL - 1][at], c % PR == 0 ? &ksc[buf][key] : nullptr);
-        store_f32(vreg[u], &vs[buf][0][at], &vs[buf][PL - 1][at], c % PR == 0 ? &vsc[buf][key] : nullptr);
+        store_f32(kreg[u], kt, &to.k[PL - 1][key * KP + d], d == 0 ? &to.kf[key] : nullptr);
+        store_f32(vreg[u], vt, &to.v[PL - 1][key * VP + d], d == 0 ? &to.vf[key] : nullptr);
       }
     }
     if constexpr (TYPE == KV_Q8) {
-      if ((int)threadIdx.x < TK) ksc[buf][threadIdx.x] = screg;
-      else if ((int)threadIdx.x < 2 * TK) vsc[buf][threadIdx.x - TK] = screg;
+      if (slot < TK) to.kf[slot] = screg;
+      constexpr int VWAVE = TK == 64 ? 1 : 0;  // the wave that holds the values' factors
+      if (rw == VWAVE) {
+        const bool factor = slot >= TK, out = factor && screg != screg && (t < blo_max || t + TK > bhi_min);
+        const bool any = __any(out);
+        if (factor) {
+          to.vf[slot - TK] = out ? 0.0f : screg;
+          if (any) to.marks[slot - TK][0] = out;
+        }
+        if (lane == 0) to.bad[0] = any;
+      }
     }
   };
 
-  auto compute = [&](int kt, int buf, int sub, bool marked) __attribute__((always_inline)) {
-    // S^T = K . Q^T: element i is key kt + 8 (i / 4) + 4 h + i % 4 of the lane's row
+  // S^T = K . Q^T of 32 keys: element i is key 8 (i / 4) + 4 h + i % 4 of the lane's row
+  auto products = [&](const Tile& x, int sub) __attribute__((always_inline)) {
     f16_t s = f16_t{};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int at = (32 * sub + col) * KP + 16 * c + 8 * h;
-      const h8_t kf = *reinterpret_cast<const h8_t*>(&ks[buf][0][at]);
-      s = mfma(kf, qhi[c], s);
-      s = mfma(kf, qlo[c], s);
-      if constexpr (PL == 2) s = mfma(*reinterpret_cast<const h8_t*>(&ks[buf][1][at]), qhi[c], s);
+      const h8_t kf = *reinterpret_cast<const h8_t*>(&x.k[0][at]);
+      h8_t q0, q1;
+      if constexpr (QL) q0 = qs[64 * c + lane], q1 = qs[64 * (NC + c) + lane];
+      else q0 = qhi[c], q1 = qlo[c];
+      s = mfma(kf, q0, s);
+      s = mfma(kf, q1, s);
+      if constexpr (PL == 2) s = mfma(*reinterpret_cast<const h8_t*>(&x.k[1][at]), q0, s);
     }
-    if constexpr (SC) {
+    return s;
+  };
+  // 16 elements' factors
+  auto times = [&](f16_t& s, const float* f) __attribute__((always_inline)) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f4_t f = *reinterpret_cast<const f4_t*>(&ksc[buf][32 * sub + 8 * q + 4 * h]);
+    for (int q = 0; q < 4; ++q) {
+      const f4_t x = *reinterpret_cast<const f4_t*>(f + 8 * q + 4 * h);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[4 * q + k] *= f[k];
-      }
+      for (int k = 0; k < 4; ++k) s[4 * q + k] *= x[k];
     }
-    float y_of = mul;  // times s: the score
-    if (capped) {
-      float far = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        s[i] *= to_cap;
-        far = fmaxf(far, fabsf(s[i]));
+  };
+  auto compute = [&](int t, const Tile& x, bool marked) __attribute__((always_inline)) {
+    f16_t s;
+    if constexpr (ahead<HD>()) s = products(x, 0);
+#pragma unroll(ahead<HD>() ? SUBS : 1)
+    for (int sub = 0; sub < SUBS; ++sub) {
+      const int kt = t + 32 * sub, key0 = kt + 4 * h;
+      if constexpr (!ahead<HD>()) {
+        if (kt >= min(k1, whi) || kt + 32 <= wlo) continue;
+        s = products(x, sub);
       }
-      if (__any(!(far < 0.9f))) {
+      if constexpr (SC) times(s, x.kf + 32 * sub);
+      float y_of = mul;  // times s: the score
+      if (capped) {
+        float far = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = fabsf(s[i]) < 0.9f ? tanh_near(s[i]) : tanh_far(s[i]);
-      } else {
+        for (int i = 0; i < 16; ++i) {
+          s[i] *= to_cap;
+          far = fmaxf(far, fabsf(s[i]));
+        }
+        if (__any(!(far < kTanhNear))) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = tanh_near(s[i]);
-      }
-    }
-    const int key0 = kt + 4 * h;
-    if (sloped) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = key0 + 8 * (i / 4) + i % 4;
-        s[i] = fmaf(s[i], mul, -slope * (float)abs(pos - key));
-      }
-      y_of = 1.0f;
-    }
-    const bool partly = kt < wlo_max || kt + 32 > whi_min;  // wave-uniform
-    uint32_t seen = 0xffffu;
-    if (partly) {
-      seen = 0;
-      const int l0 = lo - key0, h0 = hi - key0;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int k = 8 * (i / 4) + i % 4;
-        const bool in = k >= l0 && k < h0;
-        s[i] = in ? s[i] : -INFINITY;
-        seen |= (in ? 1u : 0u) << i;
-      }
-    }
-    float top = s[0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-    top *= y_of;
-    if (__any(top > m + 4.0f)) {
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const float mnew = fmaxf(m, top);
-      const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mnew);
-      m = mnew;
-      l *= alpha;
-#pragma unroll
-      for (int d = 0; d < ND; ++d) o[d] *= alpha;
-    }
-    if constexpr (SC) {
-      const float f = vsc[buf][32 * sub + col];
-      if (__any(f > D && f < INFINITY)) {
-        const float t = wave_max(f < INFINITY ? f : 0.0f);
-        const int e = min(126, (int)((__float_as_uint(t) >> 23) & 0xff) - 126);
-        const float Dnew = pow2i(e), beta = D / Dnew;
-        D = Dnew;
-        lgD = (float)e;
-        l *= beta;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) o[d] *= beta;
-      }
-    }
-    const float ref = (m == -INFINITY ? 0.0f : m) + lgD - 10.0f;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], y_of, -ref));
-      sum += s[i];
-    }
-    l += sum;
-    if constexpr (SC) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f4_t f = *reinterpret_cast<const f4_t*>(&vsc[buf][32 * sub + 8 * q + 4 * h]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) s[4 * q + k] *= f[k];
-      }
-      if (partly) {  // a factor of a key that the row does not see may be NaN
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = seen >> i & 1 ? s[i] : 0.0f;
-      }
-    }
-    // O^T += V^T . P^T, 16 keys a step: elements 8 c .. 8 c + 7 of P are the step's keys
-    // 8 (t / 4) + 4 h + t % 4, and V's are read transposed in that order
-    h8_t phi[2], plo[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int t = 0; t < 8; t += 2) {
-        h2_t x, y;
-        split2(s[8 * c + t], s[8 * c + t + 1], x, y);
-        phi[c][t] = x.x, phi[c][t + 1] = x.y, plo[c][t] = y.x, plo[c][t + 1] = y.y;
-      }
-    auto v_at = [&](int plane, int c, int d) __attribute__((always_inline)) {
-      const _Float16* p = &vs[buf][plane][(32 * sub + 16 * c + 4 * h + ((lane & 15) >> 2)) * KP + 32 * d + 16 * (lane >> 4 & 1) + 4 * (lane & 3)];
-      const h4_t x = lds_tr4(p), y = lds_tr4(p + 8 * KP);
-      return h8_t{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    };
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const h8_t vf = v_at(0, c, d);
-        o[d] = mfma(vf, phi[c], o[d]);
-        o[d] = mfma(vf, plo[c], o[d]);
-        if constexpr (PL == 2) o[d] = mfma(v_at(1, c, d), phi[c], o[d]);
-      }
-    if (marked) {  // rows that see a value that is not finite
-      const uint32_t other = (uint32_t)__shfl_xor((int)seen, 32, 64);
-      for (int k = 0; k < 32; ++k) {
-        const uint32_t half = (k >> 2 & 1) == h ? seen : other;
-        const bool in = half >> (4 * (k >> 3) + (k & 3)) & 1;
-        const uint8_t* marks = nonfinite[buf][32 * sub + k];
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int piece = 4 * d + q, c = (32 * sub + k) * PR + piece;
-            const uint32_t bits = bad[buf][c % NT / 64] ? marks[piece] >> (4 * h) : 0u;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (in && (bits >> e & 1)) o[d][4 * q + e] = __uint_as_float(0x7fc00000u);
+          for (int i = 0; i < 16; ++i) {
+            const float near = tanh_near(s[i]), out = tanh_far(s[i]);
+            s[i] = fabsf(s[i]) < kTanhNear ? near : out;
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = tanh_near(s[i]);
+        }
       }
+      if (sloped) {
+        const float away = (float)(pos - key0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = fmaf(-slope, fabsf(away - (float)(8 * (i / 4) + i % 4)), s[i] * mul);
+        y_of = 1.0f;
+      }
+      uint32_t seen = 0xffffu;
+      if (kt < wlo_max || kt + 32 > whi_min) {  // some row of the wave does not see some key
+        seen = 0;
+        const int l0 = lo - key0, h0 = hi - key0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int k = 8 * (i / 4) + i % 4;
+          const bool in = k >= l0 && k < h0;
+          s[i] = in ? s[i] : -INFINITY;
+          seen |= (in ? 1u : 0u) << i;
+        }
+      }
+      float top = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+      top *= y_of;
+      if (__any(top > m + 4.0f)) {
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float mnew = fmaxf(m, top);
+        const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mnew);
+        m = mnew;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) o[d] *= alpha;
+      }
+      if constexpr (SC) {
+        const float f = x.vf[32 * sub + col];
+        if (__any(f > D && f < INFINITY)) {
+          const float big = wave_max(f < INFINITY ? f : 0.0f);
+          const int e = min(126, (int)((__float_as_uint(big) >> 23) & 0xff) - 126);  // the next power of two
+          const float Dnew = pow2i(e), beta = D / Dnew;
+          D = Dnew;
+          lgD = (float)e;
+          l *= beta;
+#pragma unroll
+          for (int d = 0; d < ND; ++d) o[d] *= beta;
+        }
+      }
+      // from here to the end one straight line, the next 32 keys' products in it: the matrix
+      // ops run beside this part's exponentials
+      f16_t next;
+      if (ahead<HD>() && sub + 1 < SUBS) next = products(x, sub + 1);
+      const float ref = (m == -INFINITY ? 0.0f : m) + lgD - 10.0f;
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], y_of, -ref));
+        sum += s[i];
+      }
+      l += sum;
+      if constexpr (SC) times(s, x.vf + 32 * sub);
+      // O^T += V^T . P^T, 16 keys a step: elements 8 c .. 8 c + 7 of P are the step's keys
+      // 8 (t / 4) + 4 h + t % 4, and V's are read transposed in that order (the 16 lanes of
+      // a read take 4 keys x 32 bytes: rows 8 words past a multiple of 64 keep them apart)
+      auto v_at = [&](int plane, int c, int d) __attribute__((always_inline)) {
+        const _Float16* p = &x.v[plane][(32 * sub + 16 * c + 4 * h + ((lane & 15) >> 2)) * VP + 32 * d + 16 * (lane >> 4 & 1) + 4 * (lane & 3)];
+        const h4_t y = lds_tr4(p), z = lds_tr4(p + 8 * VP);
+        return h8_t{y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
+      };
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        h8_t phi, plo;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          h2_t y, z;
+          split2(s[8 * c + e], s[8 * c + e + 1], y, z);
+          phi[e] = y.x, phi[e + 1] = y.y, plo[e] = z.x, plo[e + 1] = z.y;
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+          const h8_t vf = v_at(0, c, d);
+          o[d] = mfma(vf, phi, o[d]);
+          o[d] = mfma(vf, plo, o[d]);
+          if constexpr (PL == 2) o[d] = mfma(v_at(1, c, d), phi, o[d]);
+        }
+      }
+      if (marked) {  // rows that see a value that is not finite
+        const uint32_t other = (uint32_t)__shfl_xor((int)seen, 32, 64);
+        for (int k = 0; k < 32; ++k) {
+          const uint32_t half = (k >> 2 & 1) == h ? seen : other;
+          const bool in = half >> (4 * (k >> 3) + (k & 3)) & 1;
+          const uint8_t* marks = x.marks[32 * sub + k];
+#pragma unroll
+          for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int c = TYPE == KV_Q8 ? 0 : (32 * sub + k) * PR + 4 * d + q;
+              const uint32_t bits = TYPE == KV_Q8 ? marks[0] * 15u : x.bad[c % NT / 64] ? marks[4 * d + q] >> (4 * h) : 0u;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (in && (bits >> e & 1)) o[d][4 * q + e] = __uint_as_float(0x7fc00000u);
+            }
+        }
+      }
+      if (ahead<HD>() && sub + 1 < SUBS) s = next;
     }
   };
 
   const bool busy = __any(valid);
-  if (k0 < k1) {
-    load_tile(k0);
-    store_tile(k0, 0);
-    lds_barrier();
-    int buf = 0;
-    for (int t = k0; t < k1; t += TK) {
-      const bool more = t + TK < k1;  // block-uniform
-      if (more) load_tile(t + TK);
-      bool marked = false;
-      if constexpr (TYPE != KV_Q8) {
+  const int rounds = (tile1 - tile0 + NK - 1) / NK;
+  if (mine < k1) store_tile(mine, tiles[0]);
+  if constexpr (NR > 1) lds_barrier();
+  for (int i = 0; i < rounds; ++i) {
+    const int t = mine + i * NK * TK, after = t + NK * TK;
+    const Tile& x = tiles[NB == 2 ? i & 1 : 0];
+    if (after < k1) load_tile(after);
+    bool marked = false;
 #pragma unroll
-        for (int w = 0; w < NW; ++w) marked |= __builtin_amdgcn_readfirstlane(bad[buf][w]) != 0;
-      }
-#pragma unroll
-      for (int sub = 0; sub < TK / 32; ++sub) {
-        const int kt = t + 32 * sub;
-        if (busy && kt < whi && kt + 32 > wlo && kt < k1) compute(kt, buf, sub, marked);
-      }
-      if (more) store_tile(t + TK, buf ^ 1);
-      lds_barrier();
-      buf ^= 1;
-    }
+    for (int w = 0; w < (TYPE == KV_Q8 ? 1 : NR); ++w) marked |= __builtin_amdgcn_readfirstlane(x.bad[w]) != 0;
+    if (busy && t < k1 && t < whi && t + TK > wlo) compute(t, x, marked);
+    if (after < k1) store_tile(after, tiles[NB == 2 ? (i + 1) & 1 : 0]);
+    if constexpr (NR > 1) lds_barrier();
   }
-
   l += __shfl_xor(l, 32, 64);
+
+  if constexpr (NK > 1) {
+    Merge& g = *reinterpret_cast<Merge*>(lds);
+    __syncthreads();
+    if (kg > 0) {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) g.o[kg - 1][rw][4 * d + q][lane] = f4_t{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+      g.ml[kg - 1][rw][0][lane] = m, g.ml[kg - 1][rw][1][lane] = l;
+      if (lane == 0) g.D[kg - 1][rw] = D;
+    }
+    __syncthreads();
+    if (kg > 0) return;
+    float M = m, Dm = D;
+#pragma unroll
+    for (int k = 0; k < NK - 1; ++k) M = fmaxf(M, g.ml[k][rw][0][lane]), Dm = fmaxf(Dm, g.D[k][rw]);
+    const float keep = weight_of(m, l, M) * (D / Dm);
+    l *= keep;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] *= keep;
+#pragma unroll
+    for (int k = 0; k < NK - 1; ++k) {
+      const float lk = g.ml[k][rw][1][lane], f = weight_of(g.ml[k][rw][0][lane], lk, M) * (g.D[k][rw] / Dm);
+      l += f * lk;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f4_t y = g.o[k][rw][4 * d + q][lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][4 * q + e] += f * y[e];
+        }
+    }
+    m = M, D = Dm;
+  }
   if (!valid) return;
   if (r.splits == 1 && !r.prefix) {
     const float inv = l == 0.0f ? 0.0f : (TYPE == KV_Q8 ? kQ8Unit : 1.0f) / l;
@@ -466,23 +564,38 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) k_rows_attn(RowsAt
   }
 }
 
-// Waves of a block: each takes 32 rows.
-int waves_of(int type, int64_t R) { return type == KV_F32 || R > 64 ? 4 : R > 32 ? 2 : 1; }
+// Blocks on the device at a time, by their registers and LDS.
+int64_t full_of(const RowsAttnArgs& r, int nr) {
+  const bool f32 = r.a.type == KV_F32;
+  const bool one = r.a.hd > 128 || (r.a.hd > 64 ? nr == 1 || (f32 && nr == 2) : f32 && nr == 1);
+  return (int64_t)device_cus() * (one ? 1 : 2);
+}
 
-template <int TYPE, int HD, int NW>
+// Row waves of a block: as many as leave the device full (a tile is then staged once for more
+// rows), else the fewest that the type's tiles leave room for.
+int row_waves(const RowsAttnArgs& r) {
+  const int least = r.a.hd > 128 ? (r.a.type == KV_F32 ? 4 : 2) : r.a.type == KV_F32 && r.a.hd > 64 ? 2 : 1;
+  for (int nr = 4; nr > least; nr /= 2)
+    if ((r.R + 32 * nr - 1) / (32 * nr) * r.a.n_kv >= full_of(r, nr) * 3 / 4) return nr;
+  return least;
+}
+
+template <int TYPE, int HD, int NR>
 hipError_t go(const RowsAttnArgs& r, hipStream_t s) {
-  const int64_t blocks = (r.R + 32 * NW - 1) / (32 * NW) * r.a.n_kv * r.splits;
+  const int64_t blocks = (r.R + 32 * NR - 1) / (32 * NR) * r.a.n_kv * r.splits;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
-  UAII_LAUNCH((k_rows_attn<TYPE, HD, NW>), dim3((unsigned)blocks), dim3(64 * NW), 0, s, r);
+  UAII_LAUNCH((k_rows_attn<TYPE, HD, NR>), dim3((unsigned)blocks), dim3(256), 0, s, r);
   return hipGetLastError();
 }
 
 template <int TYPE, int HD>
 hipError_t by_waves(const RowsAttnArgs& r, hipStream_t s) {
-  if constexpr (TYPE != KV_F32) {
-    const int nw = waves_of(TYPE, r.R);
-    if (nw == 1) return go<TYPE, HD, 1>(r, s);
-    if (nw == 2) return go<TYPE, HD, 2>(r, s);
+  const int nr = row_waves(r);
+  if constexpr (HD == 64 || (HD == 128 && TYPE != KV_F32)) {
+    if (nr == 1) return go<TYPE, HD, 1>(r, s);
+  }
+  if constexpr (HD < 256 || TYPE != KV_F32) {
+    if (nr == 2) return go<TYPE, HD, 2>(r, s);
   }
   return go<TYPE, HD, 4>(r, s);
 }
@@ -496,12 +609,12 @@ hipError_t by_width(const RowsAttnArgs& r, hipStream_t s) {
 
 }  // namespace
 
+// A split writes its rows' sums and the join reads them again, so there are splits only
+// where the blocks leave at least half the device idle, and of 128 keys at least.
 int rows_attn_splits(const RowsAttnArgs& r, int64_t keys) {
-  const int nw = waves_of(r.a.type, r.R);
-  const int64_t blocks = (r.R + 32 * nw - 1) / (32 * nw) * r.a.n_kv;
-  const int64_t full = (int64_t)device_cus() * (r.a.hd > 128 ? 4 : 8) / nw;
-  const int64_t most = std::min<int64_t>(128, keys / 128);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(most, r.prefix ? full / blocks : (full + blocks - 1) / blocks));
+  const int nr = row_waves(r);
+  const int64_t blocks = (r.R + 32 * nr - 1) / (32 * nr) * r.a.n_kv;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({128, (keys + 127) / 128, full_of(r, nr) / blocks}));
 }
 
 hipError_t launch_rows_attn(const RowsAttnArgs& r, hipStream_t s) {

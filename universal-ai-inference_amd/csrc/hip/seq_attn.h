@@ -16,6 +16,13 @@ typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// A pointer that all lanes share, in scalar registers.
+__device__ inline const uint8_t* uniform_at(const uint8_t* p, int64_t off) {
+  const uint64_t x = (uint64_t)p + (uint64_t)off;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+  return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
+}
+
 __device__ inline float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
 
 // Power of two that brings the largest magnitude `top` of a row into [2^14, 2^15), as an
@@ -39,13 +46,14 @@ __device__ inline h2_t q8_pair(uint32_t bytes_0_and_2) {
 }
 constexpr float kQ8Unit = 512.0f;  // 2^9: what a product of such values is multiplied by
 
-// tanh to 2 units in the last place: near 0 a quotient of polynomials (the fifth
-// convergent of tanh's continued fraction x / (1 + x^2 / (3 + x^2 / (5 + ...))), which is
-// off by less than 2^-25 up to 0.9), further out (1 - t) / (1 + t) with t = exp(-2 |x|).
+// tanh in f32, off by at most 2^-23 relative: up to kTanhNear an odd polynomial of degree
+// 11 (the smallest relative error over that range, 2^-26, by weighted least squares), further
+// out (1 - t) / (1 + t) with t = exp(-2 |x|). Scores stand mostly in the first part, and it
+// needs neither an exponential nor a quotient.
+constexpr float kTanhNear = 0.7f;
 __device__ inline float tanh_near(float x) {
-  const float x2 = x * x;
-  const float n = fmaf(x2, x2 + 105.0f, 945.0f), d = fmaf(x2, fmaf(x2, 15.0f, 420.0f), 945.0f);
-  return x * n * __builtin_amdgcn_rcpf(d);
+  const float u = x * x;
+  return x * fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -0.00508831f, 0.02002442f), -0.05352599f), 0.13328414f), -0.3333313f), 0.99999999f);
 }
 __device__ inline float tanh_far(float x) {
   const float t = __builtin_amdgcn_exp2f(-2.0f * kLog2e * fabsf(x));
@@ -55,6 +63,12 @@ __device__ inline float tanh_far(float x) {
 // Attention partials of a row: [hd] sums of p v, then the running maximum (base 2) and
 // sum of p; 4 floats for those two keep rows 16-byte aligned.
 __host__ __device__ inline int64_t part_stride(int hd) { return hd + 4; }
+
+// Weight of a partial with running maximum m and sum l; a sum that is NaN stays in.
+__device__ inline float weight_of(float m, float l, float M) {
+  if (l != l) return 1.0f;
+  return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+}
 
 // ---- rows_attn.hip: many rows over one cache -------------------------------------------
 
