@@ -6,7 +6,8 @@
 // dealt out evenly to a grid that just fills the device: a block works through the runs of
 // units that fall to it, writes a finished head's rows to the output at once, and leaves
 // the partial results of its first and last run, where a head goes on in another block,
-// to the join.
+// to the join. A batch of few units in all takes a block for each that its capacity allows,
+// and no block has to look for its share.
 #include "seq_attn.h"
 
 #include <algorithm>
@@ -25,6 +26,7 @@ struct BatchArgs {
   int* info;           // first unit of each (sequence, kv head, group), then the units of all
   const float* pre;    // partials over the prefix (RowsAttnArgs::part)
   int pre_splits, blocks;
+  int parts;           // > 0: a block for each of so many units of every head, used or not
 };
 
 __device__ inline f4_t mfma32(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -44,16 +46,17 @@ __device__ inline Span span_of(const SeqAttnArgs& a, int64_t s) {
 }
 
 template <int N>
-__device__ inline void load_words(const uint8_t* p, uint32_t (&w)[N]) {
+__device__ inline void load_words(gptr_t p, uint32_t off, uint32_t (&w)[N]) {
   if constexpr (N == 1) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
+    w[0] = load_at<uint32_t>(p, off);
   } else if constexpr (N == 2) {
-    const uint2 x = *reinterpret_cast<const uint2*>(p);
-    w[0] = x.x, w[1] = x.y;
+    typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+    const u2_t x = load_at<u2_t>(p, off);
+    w[0] = x[0], w[1] = x[1];
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
-      const u4_t x = *reinterpret_cast<const u4_t*>(p + 4 * i);
+      const u4_t x = load_at<u4_t>(p, off + 4 * i);
       w[i] = x[0], w[i + 1] = x[1], w[i + 2] = x[2], w[i + 3] = x[3];
     }
   }
@@ -90,48 +93,73 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
   const int H = a.n_kv * b.groups;
   const int n_seq = (int)a.rows;
 
-  // ---- this block's units [u, u1) of the batch's, and the sequence where they begin
-  int total;
-  {
-    const int per = (n_seq + 255) / 256, s0 = min(n_seq, tid * per), s1 = min(n_seq, s0 + per);
-    int mine = 0;
-    for (int s = s0; s < s1; ++s) mine += span_of(a, s).units();
-    int incl = mine;
+  // ---- this block's units [u, u1) of the batch's, and the sequence that holds the first
+  int s, base, u, u1;  // base: the first unit of sequence s
+  if (b.parts > 0) {
+    // few units in all: block by block, and those behind a head's last one have nothing to do
+    const int hx = (int)blockIdx.x / b.parts, uu = (int)blockIdx.x % b.parts;
+    s = hx / H;
+    const int n = span_of(a, s).units();
+    if (uu >= n) return;
+    base = 0;
+    u = hx % H * n + uu;
+    u1 = u + 1;
+  } else {
+    int total;
+    if (n_seq <= 64) {
+      // a lane for each sequence, in every wave
+      const int n = lane < n_seq ? span_of(a, lane).units() : 0;
+      int incl = n;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int x = __shfl_up(incl, o, 64);
-      incl += lane >= o ? x : 0;
-    }
-    if (lane == 63) scan[wave] = incl;
-    __syncthreads();
-    int below = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      below += w < wave ? scan[w] : 0;
-      total += scan[w];
-    }
-    total *= H;
-    if (blockIdx.x == 0 && tid == 0) b.info[(int64_t)n_seq * H] = total;
-    const int at = (int)((int64_t)total * blockIdx.x / max(1, min(b.blocks, total)));
-    int before = below + incl - mine;  // units of a head's worth of the sequences before s0
-    if (before * H <= at && at < (before + mine) * H) {
-      int s = s0;
-      for (;; ++s) {
-        const int n = span_of(a, s).units();
-        if (at < (before + n) * H) break;
-        before += n;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(incl, o, 64);
+        incl += lane >= o ? x : 0;
       }
-      found[0] = s;
-      found[1] = before;
+      total = __builtin_amdgcn_readlane(incl, 63) * H;
+      const int at = (int)((int64_t)total * blockIdx.x / max(1, min(b.blocks, total)));
+      s = __builtin_ctzll(__ballot(at < incl * H) | 1ull << 63);
+      base = (__builtin_amdgcn_readlane(incl, s) - __builtin_amdgcn_readlane(n, s)) * H;
+    } else {
+      const int per = (n_seq + 255) / 256, s0 = min(n_seq, tid * per), s1 = min(n_seq, s0 + per);
+      int mine = 0;
+      for (int i = s0; i < s1; ++i) mine += span_of(a, i).units();
+      int incl = mine;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(incl, o, 64);
+        incl += lane >= o ? x : 0;
+      }
+      if (lane == 63) scan[wave] = incl;
+      __syncthreads();
+      int below = 0;
+      total = 0;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        below += w < wave ? scan[w] : 0;
+        total += scan[w];
+      }
+      total *= H;
+      const int at = (int)((int64_t)total * blockIdx.x / max(1, min(b.blocks, total)));
+      int before = below + incl - mine;  // units of a head's worth of the sequences before s0
+      if (before * H <= at && at < (before + mine) * H) {
+        int i = s0;
+        for (;; ++i) {
+          const int n = span_of(a, i).units();
+          if (at < (before + n) * H) break;
+          before += n;
+        }
+        found[0] = i;
+        found[1] = before;
+      }
+      __syncthreads();
+      s = __builtin_amdgcn_readfirstlane(found[0]), base = __builtin_amdgcn_readfirstlane(found[1]) * H;
     }
-    __syncthreads();
+    if (blockIdx.x == 0 && tid == 0) b.info[(int64_t)n_seq * H] = total;
+    const int blocks = min(b.blocks, total);  // each has a unit at least
+    if ((int)blockIdx.x >= blocks) return;
+    u = (int)((int64_t)total * blockIdx.x / blocks);
+    u1 = (int)((int64_t)total * (blockIdx.x + 1) / blocks);
   }
-  const int blocks = min(b.blocks, total);  // each has a unit at least
-  if ((int)blockIdx.x >= blocks) return;
-  int u = (int)((int64_t)total * blockIdx.x / blocks);
-  const int u1 = (int)((int64_t)total * (blockIdx.x + 1) / blocks);
-  int s = __builtin_amdgcn_readfirstlane(found[0]), base = __builtin_amdgcn_readfirstlane(found[1]) * H;
 
   const bool capped = a.cap > 0.0f, sloped = a.slopes != nullptr;
   const int crow = PACK ? col & 7 : col;  // the lane's row of the group
@@ -149,7 +177,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
     const int kvh = hx / b.groups, head0 = kvh * b.G + hx % b.groups * RC;
     const int rows = min(RC, b.G - hx % b.groups * RC);
     const int k0 = sp.lo + UNIT * uu, k1 = min(sp.n, sp.lo + UNIT * ue);
-    if (uu == 0 && tid == 0) b.info[(int64_t)s * H + hx] = u;
+    if (b.parts == 0 && uu == 0 && tid == 0) b.info[(int64_t)s * H + hx] = u;
 
     const int64_t first = (int64_t)kvh * a.max_seq;
     const uint8_t* kbase = a.kc + (int64_t)s * a.seq_bytes;
@@ -165,7 +193,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
     // last piece, which meets zeros of q or goes to outputs that are not stored
     const uint32_t row_bytes = (uint32_t)a.hd * ES;
     auto load_keys = [&](int t) __attribute__((always_inline)) {
-      const uint8_t* kt = uniform_at(kbase, (int64_t)t * row_bytes);
+      const gptr_t kt = uniform_at(kbase, (int64_t)t * row_bytes);
       const int last = __builtin_amdgcn_readfirstlane(k1 - 1 - t);
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
@@ -173,20 +201,20 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
 #pragma unroll
         for (int w = 0; w < KW; w += 4) {
           constexpr int P = 16 / ES;
-          const u4_t y = *reinterpret_cast<const u4_t*>(kt + (kr + (uint32_t)min(g * (HD / 4) + w / 4 * P, a.hd - P) * ES));
+          const u4_t y = load_at<u4_t>(kt, kr + (uint32_t)min(g * (HD / 4) + w / 4 * P, a.hd - P) * ES);
           kw[i][w] = y[0], kw[i][w + 1] = y[1], kw[i][w + 2] = y[2], kw[i][w + 3] = y[3];
         }
       }
       if constexpr (SC) fw = (lane < 32 ? kscale : vscale)[t + min(lane & 31, last)];
     };
     auto load_values = [&](int t) __attribute__((always_inline)) {
-      const uint8_t* vt = uniform_at(vbase, (int64_t)t * row_bytes);
+      const gptr_t vt = uniform_at(vbase, (int64_t)t * row_bytes);
       const int last = __builtin_amdgcn_readfirstlane(k1 - 1 - t);
       const uint32_t d = (uint32_t)min(col * E, a.hd - E) * ES;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) load_words<VW>(vt + ((uint32_t)min(16 * i + 4 * g + r, last) * row_bytes + d), vw[i][r]);
+        for (int r = 0; r < 4; ++r) load_words<VW>(vt, (uint32_t)min(16 * i + 4 * g + r, last) * row_bytes + d, vw[i][r]);
     };
 
     // q's part of a thread (row tid / 16, E dims), ahead of the first tile, so that nothing
@@ -450,7 +478,9 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
     const bool complete = uu == 0 && ue == units;
     const int64_t stride = part_stride(a.hd);
     const bool direct = complete && b.pre_splits == 0;
-    float* part = complete ? b.whole + ((int64_t)s * H + hx) * RC * stride : b.slots + (2 * (int64_t)blockIdx.x + (uu == 0)) * RC * stride;
+    float* part = b.parts > 0 ? b.slots + (int64_t)blockIdx.x * RC * stride
+                  : complete ? b.whole + ((int64_t)s * H + hx) * RC * stride
+                             : b.slots + (2 * (int64_t)blockIdx.x + (uu == 0)) * RC * stride;
     for (int x = tid; x < rows * (a.hd / 4); x += 256) {
       const int r = x / (a.hd / 4), d = x % (a.hd / 4) * 4;
       float M = -INFINITY, den = 0.0f;
@@ -485,7 +515,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
 // eight partials of a wave at a time.
 struct JoinArgs {
   SeqAttnArgs a;
-  int G, rc, groups, blocks;
+  int G, rc, groups, blocks, parts;
   const float* slots;
   const float* whole;
   const int* info;       // null: no own keys (prompt rows)
@@ -504,20 +534,28 @@ __global__ void __launch_bounds__(64 * W) k_attn_join(JoinArgs j) {
   const int kvh = head / j.G, gr = head % j.G, H = a.n_kv * j.groups;
   const int64_t stride = part_stride(a.hd);
   // the row's own partials: those of blocks b0 .. b1, or one in `whole`
-  int own = 0, b0 = 0;
+  int own = 0;
+  int64_t ahead = 0, step = 0;  // floats from the first to the second, and from there on
   const float* at = nullptr;
   if (j.info) {
     const Span sp = span_of(a, row);
     const int units = sp.units();
     if (units > 0) {
       const int hx = kvh * j.groups + gr / j.rc;
-      const int64_t first = j.info[(int64_t)row * H + hx], total = j.info[a.rows * H];
-      // block of unit u: the last one whose first unit, total b / blocks, is not behind it
-      const int64_t blocks = min((int64_t)j.blocks, total);
-      b0 = (int)(((first + 1) * blocks - 1) / total);
-      own = (int)(((first + units) * blocks - 1) / total) - b0 + 1;
+      if (j.parts > 0) {
+        own = units;
+        at = j.slots + ((int64_t)row * H + hx) * j.parts * j.rc * stride;
+        ahead = step = j.rc * stride;
+      } else {
+        const int64_t first = j.info[(int64_t)row * H + hx], total = j.info[a.rows * H];
+        // block of unit u: the last one whose first unit, total b / blocks, is not behind it
+        const int64_t blocks = min((int64_t)j.blocks, total);
+        const int b0 = (int)(((first + 1) * blocks - 1) / total);
+        own = (int)(((first + units) * blocks - 1) / total) - b0 + 1;
+        at = own == 1 ? j.whole + ((int64_t)row * H + hx) * j.rc * stride : j.slots + (2 * (int64_t)b0 + 1) * j.rc * stride;
+        ahead = j.rc * stride, step = 2 * ahead;  // the last run of block b0, the first runs of those behind it
+      }
       if (own == 1 && j.splits == 0) return;  // written
-      at = own == 1 ? j.whole + ((int64_t)row * H + hx) * j.rc * stride : j.slots + (2 * (int64_t)b0 + 1) * j.rc * stride;
       at += gr % j.rc * stride;
     }
   }
@@ -525,7 +563,7 @@ __global__ void __launch_bounds__(64 * W) k_attn_join(JoinArgs j) {
   const float* pre = j.part + ((int64_t)kvh * R + (int64_t)row * j.G + gr) * stride;
   auto part_of = [&](int i) -> const float* {
     if (i >= own) return pre + (int64_t)(i - own) * a.n_kv * R * stride;
-    return i == 0 ? at : at + (2 * (int64_t)i - 1) * j.rc * stride;  // the blocks behind b0: their first run
+    return i == 0 ? at : at + ahead + (i - 1) * step;
   };
   const int n = own + j.splits, d = min(4 * lane, a.hd - 4);
   float m = -INFINITY, l = 0.0f;
@@ -606,7 +644,7 @@ int resident_blocks(int type, int hd, bool pack) {
 }
 
 struct Plan {
-  int G, groups, rc, blocks, splits;
+  int G, groups, rc, blocks, parts, splits;
   bool pack;
   RowsAttnArgs rows;
   size_t part, slots, whole, info;  // bytes of the scratch's parts
@@ -629,14 +667,16 @@ Plan plan_of(const SeqAttnArgs& a) {
     p.pack = a.type != KV_F32 && p.G <= 8;
     p.rc = rows_of(p.pack);
     p.groups = (p.G + p.rc - 1) / p.rc;
-    const int64_t units = a.rows * a.n_kv * p.groups * ((a.max_seq + UNIT - 1) / UNIT);
-    p.blocks = (int)std::min<int64_t>(units, resident_blocks(a.type, a.hd, p.pack));
-    p.slots = pad256(2 * (size_t)p.blocks * p.rc * row);
-    p.info = pad256(((size_t)a.rows * a.n_kv * p.groups + 1) * 4);
+    const int64_t heads = a.rows * a.n_kv * p.groups, held = a.window ? std::min<int64_t>(a.window, a.max_seq) : a.max_seq;
+    const int64_t parts = (held + UNIT - 1) / UNIT, resident = resident_blocks(a.type, a.hd, p.pack);
+    p.parts = heads * parts <= 2 * resident ? (int)parts : 0;
+    p.blocks = (int)std::min<int64_t>(heads * parts, p.parts ? 2 * resident : resident);
+    p.slots = pad256((p.parts ? 1 : 2) * (size_t)p.blocks * p.rc * row);
+    p.info = p.parts ? 0 : pad256(((size_t)heads + 1) * 4);
     if (a.n_prefix > 0) {
       p.rows.prefix = true;
       p.splits = p.rows.splits = rows_attn_splits(p.rows, a.n_prefix);
-      p.whole = pad256((size_t)a.rows * a.n_kv * p.groups * p.rc * row);
+      p.whole = p.parts ? 0 : pad256((size_t)heads * p.rc * row);
     }
   }
   p.part = pad256((size_t)p.splits * a.n_kv * p.rows.R * row);
@@ -672,6 +712,7 @@ hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
     b.pre = j.part;
     b.pre_splits = p.splits;
     b.blocks = p.blocks;
+    b.parts = p.parts;
     e = with_kernel(a.type, a.hd, p.pack, [&](auto kernel) {
       UAII_LAUNCH(kernel, dim3((unsigned)b.blocks), dim3(256), 0, s, b);
       return hipGetLastError();
@@ -680,6 +721,7 @@ hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
     j.rc = p.rc;
     j.groups = p.groups;
     j.blocks = p.blocks;
+    j.parts = p.parts;
     j.slots = b.slots;
     j.whole = b.whole;
     j.info = b.info;

@@ -23,14 +23,16 @@ __device__ inline void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-__device__ inline int wave_min_i(int v) {
-  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-  return v;
-}
+// Largest and smallest of the 64 lanes, in a scalar register.
 __device__ inline int wave_max_i(int v) {
-  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
-  return v;
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false));   // quad_perm [1,0,3,2]
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false));   // quad_perm [2,3,0,1]
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false));  // row_half_mirror
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false));  // row_mirror
+  return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
+__device__ inline int wave_min_i(int v) { return -wave_max_i(-v); }  // of values above INT32_MIN
 
 // A block has 4 waves: NR of them take 32 rows each, and the NK = 4 / NR groups of such waves
 // take the tiles of the block's keys in turn, each in an LDS region of its own.
@@ -38,14 +40,6 @@ template <int TYPE, int NR>
 constexpr int tile_keys() {
   return TYPE == KV_F32 || NR < 4 ? 32 : 64;
 }
-
-// Whether the next 32 keys' products are started beside the softmax of the last: where the
-// registers hold them.
-#ifndef UAII_AHEAD
-#define UAII_AHEAD 0
-#endif
-template <int HD>
-constexpr bool ahead() { return HD != 128 || UAII_AHEAD; }
 
 template <int TYPE, int HD, int NR>
 __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnArgs r) {
@@ -76,6 +70,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
   constexpr size_t kTiles = sizeof(Tile) * NB * NK, kMerge = NK > 1 ? sizeof(Merge) : 0;
   __shared__ __attribute__((aligned(16))) char lds[kTiles > kMerge ? kTiles : kMerge];
   __shared__ __attribute__((aligned(16))) h8_t qs[QL ? 2 * NC * 64 : 1];
+  __shared__ float qtop[QL ? NK : 1][32];
   __shared__ int rng[NR][4];
 
   const SeqAttnArgs& a = r.a;
@@ -105,18 +100,21 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
   }
   if (a.window) lo = max(lo, pos - a.window + 1);
   if (lo >= hi) lo = INT32_MAX, hi = 0;
-  const int wlo = wave_min_i(lo), wlo_max = wave_max_i(lo), whi_min = wave_min_i(hi), whi = wave_max_i(hi);
-  int blo = wlo, bhi = whi, blo_max = wlo_max, bhi_min = whi_min;
-  if constexpr (NR > 1) {
-    if (lane == 0 && kg == 0) rng[rw][0] = wlo, rng[rw][1] = wlo_max, rng[rw][2] = whi_min, rng[rw][3] = whi;
-    __syncthreads();
+  int wlo = 0, wlo_max = 0, whi_min = a.n_prefix, whi = a.n_prefix;  // over the wave's rows
+  int blo = 0, bhi = a.n_prefix, blo_max = 0, bhi_min = a.n_prefix;  // and the block's
+  if (!r.prefix || a.window) {
+    wlo = wave_min_i(lo), wlo_max = wave_max_i(lo), whi_min = wave_min_i(hi), whi = wave_max_i(hi);
+    blo = wlo, bhi = whi, blo_max = wlo_max, bhi_min = whi_min;
+    if constexpr (NR > 1) {
+      if (lane == 0 && kg == 0) rng[rw][0] = wlo, rng[rw][1] = wlo_max, rng[rw][2] = whi_min, rng[rw][3] = whi;
+      __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NR; ++w) {
-      blo = min(blo, rng[w][0]), blo_max = max(blo_max, rng[w][1]);
-      bhi_min = min(bhi_min, rng[w][2]), bhi = max(bhi, rng[w][3]);
+      for (int w = 0; w < NR; ++w) {
+        blo = min(blo, __builtin_amdgcn_readfirstlane(rng[w][0])), blo_max = max(blo_max, __builtin_amdgcn_readfirstlane(rng[w][1]));
+        bhi_min = min(bhi_min, __builtin_amdgcn_readfirstlane(rng[w][2])), bhi = max(bhi, __builtin_amdgcn_readfirstlane(rng[w][3]));
+      }
     }
   }
-  blo = __builtin_amdgcn_readfirstlane(blo), bhi = __builtin_amdgcn_readfirstlane(bhi);
   if (blo >= bhi) blo = bhi = 0;  // no row sees a key: no tiles, and none behind the end of int for a later group
   // this split's tiles
   const int n_tiles = (bhi - blo + TK - 1) / TK;
@@ -141,23 +139,23 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
   // (`slot` hides tid from the loop: its few additions again each turn, not their results in
   // registers that the products need)
   auto load_tile = [&](int t) __attribute__((always_inline)) {
-    int slot = tid;
+    uint32_t slot = tid;
     asm volatile("" : "+v"(slot));
-    const uint8_t* kt = uniform_at(kbase, (int64_t)t * row_bytes);
-    const uint8_t* vt = uniform_at(vbase, (int64_t)t * row_bytes);
+    const gptr_t kt = uniform_at(kbase, (int64_t)t * row_bytes);
+    const gptr_t vt = uniform_at(vbase, (int64_t)t * row_bytes);
     const int last = __builtin_amdgcn_readfirstlane(k1 - 1 - t);
 #pragma unroll
     for (int u = 0; u < PIECES; ++u) {
-      const int c = slot + NT * u;
-      const uint32_t off = (uint32_t)min(c / PR, last) * row_bytes + (uint32_t)min(c % PR * PE, a.hd - PE) * ES;
+      const uint32_t c = slot + NT * u;
+      const uint32_t off = min(c / PR, (uint32_t)last) * row_bytes + min(c % PR * PE, (uint32_t)(a.hd - PE)) * ES;
 #pragma unroll
       for (int w = 0; w < PW; ++w) {
-        kreg[u][w] = *reinterpret_cast<const u4_t*>(kt + off + 16 * w);
-        vreg[u][w] = *reinterpret_cast<const u4_t*>(vt + off + 16 * w);
+        kreg[u][w] = load_at<u4_t>(kt, off + 16 * w);
+        vreg[u][w] = load_at<u4_t>(vt, off + 16 * w);
       }
     }
     if constexpr (TYPE == KV_Q8) {
-      if (slot < 2 * TK) screg = (slot < TK ? kscale : vscale)[t + min(slot % TK, last)];
+      if (slot < 2 * TK) screg = (slot < TK ? kscale : vscale)[t + (int)min(slot % TK, (uint32_t)last)];
     }
   };
   const int mine = k0 + kg * TK;  // the group's first tile
@@ -167,41 +165,46 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
   float unit;  // of a raw product
   {
     const float* qp = a.q + (int64_t)query * a.ldq + (int64_t)head * a.hd;
-    float qv[NC][8], top = 0.0f;
+    constexpr int LC = QL ? NC / NK : NC;  // chunks that the wave loads: all, or its share where LDS holds q
+    auto chunk = [&](int i) { return QL ? i * NK + kg : i; };
+    float qv[LC][8], top = 0.0f;
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const float* at = qp + min(16 * c + 8 * h, a.hd - 8);
+    for (int i = 0; i < LC; ++i) {
+      const float* at = qp + min(16 * chunk(i) + 8 * h, a.hd - 8);
       const f4_t x0 = *reinterpret_cast<const f4u_t*>(at), x1 = *reinterpret_cast<const f4u_t*>(at + 4);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) qv[c][k] = k < 4 ? x0[k] : x1[k - 4];
+      for (int k = 0; k < 8; ++k) qv[i][k] = k < 4 ? x0[k] : x1[k - 4];
     }
     // behind q, so that nothing waits for the tile with it
     if (mine < k1) load_tile(mine);
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int i = 0; i < LC; ++i)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        qv[c][k] = 16 * c + 8 * h < a.hd ? qv[c][k] * a.scale : 0.0f;
-        top = fmaxf(top, fabsf(qv[c][k]));
+        qv[i][k] = 16 * chunk(i) + 8 * h < a.hd ? qv[i][k] * a.scale : 0.0f;
+        top = fmaxf(top, fabsf(qv[i][k]));
       }
     top = fmaxf(top, __shfl_xor(top, 32, 64));
+    if constexpr (QL) {
+      qtop[kg][col] = top;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < NK; ++w) top = fmaxf(top, qtop[w][col]);
+    }
     const int e = row_exponent(top);
     const float up = pow2i(e);
     unit = pow2i(-e) * (TYPE == KV_Q8 ? kQ8Unit : 1.0f);
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
+    for (int i = 0; i < LC; ++i) {
       h8_t hi8, lo8;
 #pragma unroll
       for (int k = 0; k < 8; k += 2) {
         h2_t x, y;
-        split2(qv[c][k] * up, qv[c][k + 1] * up, x, y);
+        split2(qv[i][k] * up, qv[i][k + 1] * up, x, y);
         hi8[k] = x.x, hi8[k + 1] = x.y, lo8[k] = y.x, lo8[k + 1] = y.y;
       }
-      if constexpr (QL) {
-        if (c % NK == kg) qs[64 * c + lane] = hi8, qs[64 * (NC + c) + lane] = lo8;
-      } else {
-        qhi[c] = hi8, qlo[c] = lo8;
-      }
+      if constexpr (QL) qs[64 * chunk(i) + lane] = hi8, qs[64 * (NC + chunk(i)) + lane] = lo8;
+      else qhi[i] = hi8, qlo[i] = lo8;
     }
     if constexpr (QL) __syncthreads();
   }
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
     }
   };
   auto store_tile = [&](int t, Tile& to) __attribute__((always_inline)) {
-    int slot = tid;
+    uint32_t slot = tid;
     asm volatile("" : "+v"(slot));
     // Where some row does not see some key, a probability of 0 must not meet a value that is
     // not finite: such values are stored as 0 and marked.
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
         if (any) {
 #pragma unroll
           for (int u = 0; u < PIECES; ++u) {
-            const int c = slot + NT * u;
+            const uint32_t c = slot + NT * u;
             uint32_t bits = 0;
 #pragma unroll
             for (int w = 0; w < 4 * PW; ++w) {
@@ -287,7 +290,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
     }
 #pragma unroll
     for (int u = 0; u < PIECES; ++u) {
-      const int c = slot + NT * u, key = c / PR, d = c % PR * PE;
+      const uint32_t c = slot + NT * u, key = c / PR, d = c % PR * PE;
       _Float16 *kt = &to.k[0][key * KP + d], *vt = &to.v[0][key * VP + d];
       if constexpr (TYPE == KV_F16) {
         *reinterpret_cast<u4_t*>(kt) = kreg[u][0];
@@ -352,15 +355,11 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
     }
   };
   auto compute = [&](int t, const Tile& x, bool marked) __attribute__((always_inline)) {
-    f16_t s;
-    if constexpr (ahead<HD>()) s = products(x, 0);
-#pragma unroll(ahead<HD>() ? SUBS : 1)
+#pragma unroll 1
     for (int sub = 0; sub < SUBS; ++sub) {
       const int kt = t + 32 * sub, key0 = kt + 4 * h;
-      if constexpr (!ahead<HD>()) {
-        if (kt >= min(k1, whi) || kt + 32 <= wlo) continue;
-        s = products(x, sub);
-      }
+      if (kt >= min(k1, whi) || kt + 32 <= wlo) continue;
+      f16_t s = products(x, sub);
       if constexpr (SC) times(s, x.kf + 32 * sub);
       float y_of = mul;  // times s: the score
       if (capped) {
@@ -425,18 +424,14 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
           for (int d = 0; d < ND; ++d) o[d] *= beta;
         }
       }
-      // from here to the end one straight line, the next 32 keys' products in it: the matrix
-      // ops run beside this part's exponentials
-      f16_t next;
-      if (ahead<HD>() && sub + 1 < SUBS) next = products(x, sub + 1);
       const float ref = (m == -INFINITY ? 0.0f : m) + lgD - 10.0f;
-      float sum = 0.0f;
+      f4_t sum = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], y_of, -ref));
-        sum += s[i];
+        sum[i % 4] += s[i];
       }
-      l += sum;
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       if constexpr (SC) times(s, x.vf + 32 * sub);
       // O^T += V^T . P^T, 16 keys a step: elements 8 c .. 8 c + 7 of P are the step's keys
       // 8 (t / 4) + 4 h + t % 4, and V's are read transposed in that order (the 16 lanes of
@@ -481,7 +476,6 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
             }
         }
       }
-      if (ahead<HD>() && sub + 1 < SUBS) s = next;
     }
   };
 

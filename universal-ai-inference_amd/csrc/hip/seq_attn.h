@@ -16,11 +16,19 @@ typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 
-// A pointer that all lanes share, in scalar registers.
-__device__ inline const uint8_t* uniform_at(const uint8_t* p, int64_t off) {
+// Global memory at p + off, p being the same in all lanes: the address in scalar registers.
+// (Through the address space: a generic pointer's loads would count as LDS reads too, and
+// each wait for LDS would wait for them.)
+#define UAII_GLOBAL __attribute__((address_space(1)))
+typedef const UAII_GLOBAL uint8_t* gptr_t;
+__device__ inline gptr_t uniform_at(const uint8_t* p, int64_t off) {
   const uint64_t x = (uint64_t)p + (uint64_t)off;
   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
-  return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
+  return reinterpret_cast<gptr_t>((uint64_t)hi << 32 | lo);
+}
+template <typename T>
+__device__ inline T load_at(gptr_t p, uint32_t off) {
+  return *reinterpret_cast<const UAII_GLOBAL T*>(p + off);
 }
 
 __device__ inline float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 <= e <= 127
@@ -34,8 +42,10 @@ __device__ inline int row_exponent(float top) {
 
 // Two f32 as f16 pairs hi + lo, about 22 significant bits together.
 __device__ inline void split2(float a, float b, h2_t& hi, h2_t& lo) {
+  float minus = -1.0f;  // not known to be -1: the remainder is then one mixed-precision FMA, no conversion and subtraction
+  asm("" : "+s"(minus));
   hi = __builtin_convertvector((f2_t{a, b}), h2_t);
-  lo = __builtin_convertvector((f2_t{fmaf((float)hi.x, -1.0f, a), fmaf((float)hi.y, -1.0f, b)}), h2_t);
+  lo = __builtin_convertvector((f2_t{fmaf((float)hi.x, minus, a), fmaf((float)hi.y, minus, b)}), h2_t);
 }
 
 // The 8-bit values of a word, (byte - 128) 2^-9 in f16: the byte as an f16 subnormal
