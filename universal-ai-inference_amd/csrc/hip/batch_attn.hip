@@ -661,7 +661,7 @@ Plan plan_of(const SeqAttnArgs& a) {
   p.rows.G = p.G;
   p.rows.R = a.rows * p.G;
   if (!a.n_keys) {
-    p.rows.splits = rows_attn_splits(p.rows, (int64_t)a.p0 + a.rows);
+    rows_attn_shape(&p.rows);
     p.splits = p.rows.splits > 1 ? p.rows.splits : 0;
   } else {
     p.pack = a.type != KV_F32 && p.G <= 8;
@@ -675,7 +675,8 @@ Plan plan_of(const SeqAttnArgs& a) {
     p.info = p.parts ? 0 : pad256(((size_t)heads + 1) * 4);
     if (a.n_prefix > 0) {
       p.rows.prefix = true;
-      p.splits = p.rows.splits = rows_attn_splits(p.rows, a.n_prefix);
+      rows_attn_shape(&p.rows);
+      p.splits = p.rows.splits;
       p.whole = p.parts ? 0 : pad256((size_t)heads * p.rc * row);
     }
   }

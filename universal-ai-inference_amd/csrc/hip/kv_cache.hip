@@ -18,6 +18,7 @@
 #include "kv_cache.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace uaii_hip {
 namespace {
@@ -52,11 +53,16 @@ __device__ inline Place place_of(const KvRowsArgs& a, uint32_t unit, uint32_t un
   return p;
 }
 
-// Largest of the GS lanes of a group.
+// Largest of the GS lanes of a group, on DPP moves within 16 lanes.
 template <int GS>
 __device__ inline uint32_t group_max(uint32_t v) {
-#pragma unroll
-  for (int o = GS / 2; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+  auto dpp = [&](auto ctrl) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, false); };
+  v = max(v, dpp(std::integral_constant<int, 0xB1>{}));                          // quad_perm [1,0,3,2]
+  v = max(v, dpp(std::integral_constant<int, 0x4E>{}));                          // quad_perm [2,3,0,1]
+  if constexpr (GS >= 8) v = max(v, dpp(std::integral_constant<int, 0x141>{}));  // row_half_mirror
+  if constexpr (GS >= 16) v = max(v, dpp(std::integral_constant<int, 0x140>{}));  // row_mirror
+  if constexpr (GS >= 32) v = max(v, (uint32_t)__shfl_xor((int)v, 16, 64));
+  if constexpr (GS >= 64) v = max(v, (uint32_t)__shfl_xor((int)v, 32, 64));
   return v;
 }
 

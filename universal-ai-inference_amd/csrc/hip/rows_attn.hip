@@ -3,11 +3,13 @@
 #include "seq_attn.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace uaii_hip {
 namespace {
 
 __device__ inline f16_t mfma(h8_t a, h8_t b, f16_t c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ inline f4_t mfma(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 // Four f16 of the transposed 4 x 16 piece that a group of 16 lanes names (8 bytes each).
 __device__ inline h4_t lds_tr4(const _Float16* p) {
@@ -34,22 +36,31 @@ __device__ inline int wave_max_i(int v) {
 }
 __device__ inline int wave_min_i(int v) { return -wave_max_i(-v); }  // of values above INT32_MIN
 
-// A block has 4 waves: NR of them take 32 rows each, and the NK = 4 / NR groups of such waves
+// A block has 4 waves: NR of them take MR rows each, and the NK = 4 / NR groups of such waves
 // take the tiles of the block's keys in turn, each in an LDS region of its own.
-template <int TYPE, int NR>
+//
+// MR is 32, on the 32x32 matrix ops, where a fragment of keys or values read from LDS serves
+// twice as many rows; the rows' queries and sums take HD registers of a lane, which at
+// head_dim 256 leaves none: 16 rows there, on the 16x16 ops.
+constexpr int row_tile(int hd) { return hd > 128 ? 16 : 32; }
+template <int TYPE, int HD, int NR>
 constexpr int tile_keys() {
-  return TYPE == KV_F32 || NR < 4 ? 32 : 64;
+  return TYPE == KV_Q8 && HD == 64 && NR == 4 ? 64 : 32;  // a piece for each thread
 }
 
 template <int TYPE, int HD, int NR>
-__global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnArgs r) {
-  constexpr int NK = 4 / NR, NT = 64 * NR, TK = tile_keys<TYPE, NR>(), SUBS = TK / 32;
+__global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
+  constexpr int NK = 4 / NR, NT = 64 * NR, TK = tile_keys<TYPE, HD, NR>(), SUBS = TK / 32;
+  constexpr int MR = row_tile(HD), GL = 64 / MR;        // lane groups: lanes of a row
+  constexpr int NE = 32 / GL, KS = MR == 32 ? 8 : 16;   // scores of a lane for 32 keys: element i is key KS (i / 4) + 4 h + i % 4
   constexpr int NB = NR == 1 ? 1 : 2;                   // buffers of a region; a lone wave needs one
   constexpr bool QL = NR == 1;                          // q's fragments in LDS: the waves share their rows
   constexpr int PL = TYPE == KV_F32 ? 2 : 1;            // f16 planes of a tile (hi, lo)
   constexpr bool SC = TYPE != KV_F16;                   // a factor for each key
   constexpr int KP = HD + 8, VP = HD + 16;              // rows of a tile (halfs): see v_at
-  constexpr int NC = HD / 16, ND = HD / 32;             // dim chunks of S, dim tiles of O
+  constexpr int CD = 8 * GL, NC = HD / CD, ND = HD / MR;  // dim chunks of S, dim tiles of O
+  constexpr int NQ = MR / (4 * GL);                     // runs of 4 dims that a lane has of an O tile: MR d + KS q + 4 h
+  using Acc = std::conditional_t<MR == 32, f16_t, f4_t>;
   constexpr int PE = TYPE == KV_Q8 ? 16 : 8;            // dims of a staged piece
   constexpr int PR = HD / PE;                           // pieces of a key's row
   constexpr int PIECES = TK * PR / NT;
@@ -58,31 +69,34 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
     __attribute__((aligned(16))) _Float16 k[PL][TK * KP];
     __attribute__((aligned(16))) _Float16 v[PL][TK * VP];
     __attribute__((aligned(16))) float kf[SC ? TK : 4], vf[SC ? TK : 4];
-    // values that are not finite: a bit a dim (KV_Q8: one for the row), and whether a wave's
-    // pieces have one (KV_Q8: whether the tile has)
-    uint8_t marks[TK][TYPE == KV_Q8 ? 1 : HD / 8];
-    int bad[TYPE == KV_Q8 ? 1 : NR];
+  };
+  // values of a tile that are not finite: a bit a dim (KV_Q8: one for the row), and whether a
+  // wave's pieces have one (KV_Q8: whether the tile has); of this tile and the next
+  struct Marks {
+    uint8_t at[TK][TYPE == KV_Q8 ? 1 : HD / 8];
+    int any[TYPE == KV_Q8 ? 1 : NR];
   };
   struct Merge {  // of the groups behind the first
-    f4_t o[NK > 1 ? NK - 1 : 1][NR][HD / 8][64];
+    f4_t o[NK > 1 ? NK - 1 : 1][NR][ND * NQ][64];
     float ml[NK > 1 ? NK - 1 : 1][NR][2][64], D[NK > 1 ? NK - 1 : 1][NR];
   };
   constexpr size_t kTiles = sizeof(Tile) * NB * NK, kMerge = NK > 1 ? sizeof(Merge) : 0;
   __shared__ __attribute__((aligned(16))) char lds[kTiles > kMerge ? kTiles : kMerge];
+  __shared__ Marks marks[NK][2];
   __shared__ __attribute__((aligned(16))) h8_t qs[QL ? 2 * NC * 64 : 1];
-  __shared__ float qtop[QL ? NK : 1][32];
+  __shared__ float qtop[QL ? NK : 1][MR];
   __shared__ int rng[NR][4];
 
   const SeqAttnArgs& a = r.a;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rw = wave % NR, kg = wave / NR, tid = threadIdx.x - NT * kg;
-  const int lane = threadIdx.x & 63, col = lane & 31, h = lane >> 5;
+  const int lane = threadIdx.x & 63, col = lane % MR, h = lane / MR;
   Tile* tiles = reinterpret_cast<Tile*>(lds) + NB * kg;
   const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv);
   const int sx = (int)(blockIdx.x / (unsigned)a.n_kv);
   const int split = sx % r.splits;
-  const int nx = (int)((r.R + 32 * NR - 1) / (32 * NR));
-  const int64_t row_at = (int64_t)(nx - 1 - sx / r.splits) * (32 * NR) + 32 * rw + col;  // the longest first
+  const int nx = (int)((r.R + MR * NR - 1) / (MR * NR));
+  const int64_t row_at = (int64_t)(nx - 1 - sx / r.splits) * (MR * NR) + MR * rw + col;  // the longest first
   const bool valid = row_at < r.R;
   const int64_t row = valid ? row_at : r.R - 1;
   const int query = (int)(row / r.G), head = kvh * r.G + (int)(row % r.G);
@@ -160,7 +174,11 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
   };
   const int mine = k0 + kg * TK;  // the group's first tile
 
-  // q * scale * 2^e as f16 hi + lo: the lane has dims 16 c + 8 h .. + 7 of its row
+  auto row_max = [](float v) __attribute__((always_inline)) {  // over a row's lanes
+    if constexpr (MR == 16) v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+  };
+  // q * scale * 2^e as f16 hi + lo: the lane has dims CD c + 8 h .. + 7 of its row
   h8_t qhi[QL ? 1 : NC], qlo[QL ? 1 : NC];
   float unit;  // of a raw product
   {
@@ -170,7 +188,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
     float qv[LC][8], top = 0.0f;
 #pragma unroll
     for (int i = 0; i < LC; ++i) {
-      const float* at = qp + min(16 * chunk(i) + 8 * h, a.hd - 8);
+      const float* at = qp + min(CD * chunk(i) + 8 * h, a.hd - 8);
       const f4_t x0 = *reinterpret_cast<const f4u_t*>(at), x1 = *reinterpret_cast<const f4u_t*>(at + 4);
 #pragma unroll
       for (int k = 0; k < 8; ++k) qv[i][k] = k < 4 ? x0[k] : x1[k - 4];
@@ -181,10 +199,10 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
     for (int i = 0; i < LC; ++i)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        qv[i][k] = 16 * chunk(i) + 8 * h < a.hd ? qv[i][k] * a.scale : 0.0f;
+        qv[i][k] = CD * chunk(i) + 8 * h < a.hd ? qv[i][k] * a.scale : 0.0f;
         top = fmaxf(top, fabsf(qv[i][k]));
       }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    top = row_max(top);
     if constexpr (QL) {
       qtop[kg][col] = top;
       __syncthreads();
@@ -215,9 +233,9 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
 
   // The lane's row: probabilities are 2^(y - m + 10) / D. m follows the maximum in steps (a
   // score may pass it by 2^4), D is a power of two over the values' factors so far.
-  f16_t o[ND];
+  Acc o[ND];
 #pragma unroll
-  for (int d = 0; d < ND; ++d) o[d] = f16_t{};
+  for (int d = 0; d < ND; ++d) o[d] = Acc{};
   float m = -INFINITY, l = 0.0f, D = SC ? 0x1p-60f : 1.0f, lgD = SC ? -60.0f : 0.0f;
 
   // f32 pieces: rows scaled to their largest finite magnitude, as hi + lo
@@ -246,48 +264,57 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
       if (factor) *factor = pow2i(-e);
     }
   };
-  auto store_tile = [&](int t, Tile& to) __attribute__((always_inline)) {
-    uint32_t slot = tid;
-    asm volatile("" : "+v"(slot));
-    // Where some row does not see some key, a probability of 0 must not meet a value that is
-    // not finite: such values are stored as 0 and marked.
-    if constexpr (TYPE != KV_Q8) {
-      bool any = false;
-      if (t < blo_max || t + TK > bhi_min) {
-        uint32_t top = 0;
+  // Where some row does not see some key, a probability of 0 must not meet a value that is not
+  // finite: such values (KV_Q8: factors) are stored as 0 and marked.
+  auto partly = [&](int t) __attribute__((always_inline)) { return t < blo_max || t + TK > bhi_min; };
+  auto mark = [&](Marks& to) __attribute__((always_inline)) {
+    if constexpr (TYPE == KV_Q8) {
+      constexpr int VWAVE = TK == 64 ? 1 : 0;  // the wave that holds the values' factors
+      if (rw == VWAVE) {
+        const bool factor = tid >= TK, out = factor && screg != screg;
+        const bool any = __any(out);
+        if (factor) to.at[tid - TK][0] = out;
+        screg = out ? 0.0f : screg;
+        if (lane == 0) to.any[0] = any;
+      }
+    } else {
+      uint32_t top = 0;
 #pragma unroll
-        for (int u = 0; u < PIECES; ++u)
+      for (int u = 0; u < PIECES; ++u)
+#pragma unroll
+        for (int w = 0; w < 4 * PW; ++w) {
+          const uint32_t x = vreg[u][w / 4][w % 4];
+          top = TYPE == KV_F16 ? max(top, max(x & 0x7fffu, x >> 16 & 0x7fffu)) : max(top, (x & 0x7fffffffu) >> 16);
+        }
+      const bool any = __any(top >= (TYPE == KV_F16 ? 0x7c00u : 0x7f80u));
+      if (any) {
+#pragma unroll
+        for (int u = 0; u < PIECES; ++u) {
+          const uint32_t c = tid + NT * u;
+          uint32_t bits = 0;
 #pragma unroll
           for (int w = 0; w < 4 * PW; ++w) {
-            const uint32_t x = vreg[u][w / 4][w % 4];
-            top = TYPE == KV_F16 ? max(top, max(x & 0x7fffu, x >> 16 & 0x7fffu)) : max(top, (x & 0x7fffffffu) >> 16);
-          }
-        any = __any(top >= (TYPE == KV_F16 ? 0x7c00u : 0x7f80u));
-        if (any) {
-#pragma unroll
-          for (int u = 0; u < PIECES; ++u) {
-            const uint32_t c = slot + NT * u;
-            uint32_t bits = 0;
-#pragma unroll
-            for (int w = 0; w < 4 * PW; ++w) {
-              uint32_t x = vreg[u][w / 4][w % 4];
-              if constexpr (TYPE == KV_F16) {
-                const bool x0 = (x & 0x7c00u) == 0x7c00u, x1 = (x & 0x7c000000u) == 0x7c000000u;
-                bits |= (x0 ? 1u : 0u) << (2 * w) | (x1 ? 2u : 0u) << (2 * w);
-                x &= (x0 ? 0u : 0xffffu) | (x1 ? 0u : 0xffff0000u);
-              } else {
-                const bool out = (x & 0x7f800000u) == 0x7f800000u;
-                bits |= (out ? 1u : 0u) << w;
-                x = out ? 0u : x;
-              }
-              vreg[u][w / 4][w % 4] = x;
+            uint32_t x = vreg[u][w / 4][w % 4];
+            if constexpr (TYPE == KV_F16) {
+              const bool x0 = (x & 0x7c00u) == 0x7c00u, x1 = (x & 0x7c000000u) == 0x7c000000u;
+              bits |= (x0 ? 1u : 0u) << (2 * w) | (x1 ? 2u : 0u) << (2 * w);
+              x &= (x0 ? 0u : 0xffffu) | (x1 ? 0u : 0xffff0000u);
+            } else {
+              const bool out = (x & 0x7f800000u) == 0x7f800000u;
+              bits |= (out ? 1u : 0u) << w;
+              x = out ? 0u : x;
             }
-            to.marks[c / PR][c % PR] = (uint8_t)bits;
+            vreg[u][w / 4][w % 4] = x;
           }
+          to.at[c / PR][c % PR] = (uint8_t)bits;
         }
       }
-      if (lane == 0) to.bad[rw] = any;
+      if (lane == 0) to.any[rw] = any;
     }
+  };
+  auto store_tile = [&](Tile& to) __attribute__((always_inline)) {
+    uint32_t slot = tid;
+    asm volatile("" : "+v"(slot));
 #pragma unroll
     for (int u = 0; u < PIECES; ++u) {
       const uint32_t c = slot + NT * u, key = c / PR, d = c % PR * PE;
@@ -315,84 +342,105 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
       }
     }
     if constexpr (TYPE == KV_Q8) {
-      if (slot < TK) to.kf[slot] = screg;
-      constexpr int VWAVE = TK == 64 ? 1 : 0;  // the wave that holds the values' factors
-      if (rw == VWAVE) {
-        const bool factor = slot >= TK, out = factor && screg != screg && (t < blo_max || t + TK > bhi_min);
-        const bool any = __any(out);
-        if (factor) {
-          to.vf[slot - TK] = out ? 0.0f : screg;
-          if (any) to.marks[slot - TK][0] = out;
-        }
-        if (lane == 0) to.bad[0] = any;
-      }
+      if (slot < 2 * TK) *(slot < TK ? &to.kf[slot] : &to.vf[slot - TK]) = screg;
     }
   };
 
-  // S^T = K . Q^T of 32 keys: element i is key 8 (i / 4) + 4 h + i % 4 of the lane's row
-  auto products = [&](const Tile& x, int sub) __attribute__((always_inline)) {
-    f16_t s = f16_t{};
+  // S^T = K . Q^T of 32 keys
+  // (`loads`: global loads beside them, of the next tile)
+  auto products = [&](const Tile& x, int sub, float (&s)[NE], auto loads) __attribute__((always_inline)) {
+    constexpr int KT = 32 / MR;  // key tiles
+    Acc acc[KT];
+#pragma unroll
+    for (int i = 0; i < KT; ++i) acc[i] = Acc{};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int at = (32 * sub + col) * KP + 16 * c + 8 * h;
-      const h8_t kf = *reinterpret_cast<const h8_t*>(&x.k[0][at]);
       h8_t q0, q1;
       if constexpr (QL) q0 = qs[64 * c + lane], q1 = qs[64 * (NC + c) + lane];
       else q0 = qhi[c], q1 = qlo[c];
-      s = mfma(kf, q0, s);
-      s = mfma(kf, q1, s);
-      if constexpr (PL == 2) s = mfma(*reinterpret_cast<const h8_t*>(&x.k[1][at]), q0, s);
-    }
-    return s;
-  };
-  // 16 elements' factors
-  auto times = [&](f16_t& s, const float* f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const f4_t x = *reinterpret_cast<const f4_t*>(f + 8 * q + 4 * h);
+      for (int i = 0; i < KT; ++i) {
+        const int at = (32 * sub + MR * i + col) * KP + CD * c + 8 * h;
+        const h8_t kf = *reinterpret_cast<const h8_t*>(&x.k[0][at]);
+        acc[i] = mfma(kf, q0, acc[i]);
+        acc[i] = mfma(kf, q1, acc[i]);
+        if constexpr (PL == 2) acc[i] = mfma(*reinterpret_cast<const h8_t*>(&x.k[1][at]), q0, acc[i]);
+      }
+    }
+    // The order: fragments are read AHEAD steps before their matrix ops, and the loads stand
+    // between the ops, where the wave would only wait (issued together they hold it up: a load
+    // of 64 x 16 bytes takes the CU's vector memory path 16 cycles, and four waves share it).
+    constexpr int OPS = PL == 2 ? 3 : 2, READS = PL, Q = QL ? 2 : 0, STEPS = NC * KT, AHEAD = STEPS > 4 ? 3 : 1;
+    constexpr int LOADS = (decltype(loads)::value + STEPS - 1) / STEPS;
+    __builtin_amdgcn_sched_group_barrier(0x100, (READS + Q) * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < STEPS - AHEAD; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, OPS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, READS + Q, 0);
+      if constexpr (LOADS > 0) __builtin_amdgcn_sched_group_barrier(0x20, LOADS, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x8, OPS, 0);
+      if constexpr (LOADS > 0) __builtin_amdgcn_sched_group_barrier(0x20, LOADS, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < NE; ++i) s[i] = acc[i / (NE / KT)][i % (NE / KT)];
+  };
+  // the factors of a lane's keys
+  auto times = [&](float (&s)[NE], const float* f) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < NE / 4; ++q) {
+      const f4_t x = *reinterpret_cast<const f4_t*>(f + KS * q + 4 * h);
 #pragma unroll
       for (int k = 0; k < 4; ++k) s[4 * q + k] *= x[k];
     }
   };
-  auto compute = [&](int t, const Tile& x, bool marked) __attribute__((always_inline)) {
-#pragma unroll 1
+  // One tile, the next one's way to its place (`to`, `note`) beside it.
+  auto compute = [&](int t, const Tile& x, const Marks& known, bool marked, int next, Tile& to, Marks& note) __attribute__((always_inline)) {
+#pragma unroll
     for (int sub = 0; sub < SUBS; ++sub) {
       const int kt = t + 32 * sub, key0 = kt + 4 * h;
-      if (kt >= min(k1, whi) || kt + 32 <= wlo) continue;
-      f16_t s = products(x, sub);
+      float s[NE];
+      if (sub == 0) {
+        load_tile(next);
+        products(x, sub, s, std::integral_constant<int, 2 * PIECES * PW + (TYPE == KV_Q8)>{});
+      } else {
+        products(x, sub, s, std::integral_constant<int, 0>{});
+      }
       if constexpr (SC) times(s, x.kf + 32 * sub);
       float y_of = mul;  // times s: the score
       if (capped) {
         float far = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < NE; ++i) {
           s[i] *= to_cap;
           far = fmaxf(far, fabsf(s[i]));
         }
         if (__any(!(far < kTanhNear))) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < NE; ++i) {
             const float near = tanh_near(s[i]), out = tanh_far(s[i]);
             s[i] = fabsf(s[i]) < kTanhNear ? near : out;
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = tanh_near(s[i]);
+          for (int i = 0; i < NE; ++i) s[i] = tanh_near(s[i]);
         }
       }
       if (sloped) {
         const float away = (float)(pos - key0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = fmaf(-slope, fabsf(away - (float)(8 * (i / 4) + i % 4)), s[i] * mul);
+        for (int i = 0; i < NE; ++i) s[i] = fmaf(-slope, fabsf(away - (float)(KS * (i / 4) + i % 4)), s[i] * mul);
         y_of = 1.0f;
       }
-      uint32_t seen = 0xffffu;
+      uint32_t seen = (1u << NE) - 1;
       if (kt < wlo_max || kt + 32 > whi_min) {  // some row of the wave does not see some key
         seen = 0;
         const int l0 = lo - key0, h0 = hi - key0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int k = 8 * (i / 4) + i % 4;
+        for (int i = 0; i < NE; ++i) {
+          const int k = KS * (i / 4) + i % 4;
           const bool in = k >= l0 && k < h0;
           s[i] = in ? s[i] : -INFINITY;
           seen |= (in ? 1u : 0u) << i;
@@ -400,10 +448,10 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
       }
       float top = s[0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+      for (int i = 1; i < NE; ++i) top = fmaxf(top, s[i]);
       top *= y_of;
       if (__any(top > m + 4.0f)) {
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        top = row_max(top);
         const float mnew = fmaxf(m, top);
         const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mnew);
         m = mnew;
@@ -412,7 +460,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
         for (int d = 0; d < ND; ++d) o[d] *= alpha;
       }
       if constexpr (SC) {
-        const float f = x.vf[32 * sub + col];
+        const float f = x.vf[32 * sub + (lane & 31)];
         if (__any(f > D && f < INFINITY)) {
           const float big = wave_max(f < INFINITY ? f : 0.0f);
           const int e = min(126, (int)((__float_as_uint(big) >> 23) & 0xff) - 126);  // the next power of two
@@ -424,25 +472,27 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
           for (int d = 0; d < ND; ++d) o[d] *= beta;
         }
       }
+      if (sub + 1 == SUBS && partly(next)) mark(note);
       const float ref = (m == -INFINITY ? 0.0f : m) + lgD - 10.0f;
       f4_t sum = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < NE; ++i) {
         s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], y_of, -ref));
         sum[i % 4] += s[i];
       }
       l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
       if constexpr (SC) times(s, x.vf + 32 * sub);
-      // O^T += V^T . P^T, 16 keys a step: elements 8 c .. 8 c + 7 of P are the step's keys
-      // 8 (t / 4) + 4 h + t % 4, and V's are read transposed in that order (the 16 lanes of
-      // a read take 4 keys x 32 bytes: rows 8 words past a multiple of 64 keep them apart)
+      // O^T += V^T . P^T: elements 8 c .. 8 c + 7 of P are the keys of a step (16, or 32 with
+      // 16 rows), in the order in which V is read, transposed: the 16 lanes of a read take 4
+      // keys x 32 bytes, which rows 8 words past a multiple of 64 keep in banks of their own
       auto v_at = [&](int plane, int c, int d) __attribute__((always_inline)) {
-        const _Float16* p = &x.v[plane][(32 * sub + 16 * c + 4 * h + ((lane & 15) >> 2)) * VP + 32 * d + 16 * (lane >> 4 & 1) + 4 * (lane & 3)];
-        const h4_t y = lds_tr4(p), z = lds_tr4(p + 8 * VP);
+        const int key = 32 * sub + 16 * c + 4 * h + ((lane & 15) >> 2), dim = MR * d + 4 * (lane & 3) + (MR == 32 ? 16 * (lane >> 4 & 1) : 0);
+        const _Float16* p = &x.v[plane][key * VP + dim];
+        const h4_t y = lds_tr4(p), z = lds_tr4(p + KS * VP);
         return h8_t{y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
       };
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
+      for (int c = 0; c < NE / 8; ++c) {
         h8_t phi, plo;
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
@@ -458,18 +508,34 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
           if constexpr (PL == 2) o[d] = mfma(v_at(1, c, d), phi, o[d]);
         }
       }
+      if (sub + 1 == SUBS) store_tile(to);
+      {
+        constexpr int OPS = PL == 2 ? 3 : 2, READS = 2 * PL, STEPS = NE / 8 * ND, AHEAD = STEPS > 4 ? 3 : 2;
+        constexpr int WRITES = (2 * PIECES * (TYPE == KV_F16 ? 1 : 2) + (TYPE == KV_Q8) + AHEAD - 1) / AHEAD;
+        __builtin_amdgcn_sched_group_barrier(0x100, READS * AHEAD, 1);
+#pragma unroll
+        for (int i = 0; i < STEPS - AHEAD; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, OPS, 1);
+          __builtin_amdgcn_sched_group_barrier(0x100, READS, 1);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x8, OPS, 1);
+          if (sub + 1 == SUBS) __builtin_amdgcn_sched_group_barrier(0x200, WRITES, 1);
+        }
+      }
       if (marked) {  // rows that see a value that is not finite
-        const uint32_t other = (uint32_t)__shfl_xor((int)seen, 32, 64);
         for (int k = 0; k < 32; ++k) {
-          const uint32_t half = (k >> 2 & 1) == h ? seen : other;
-          const bool in = half >> (4 * (k >> 3) + (k & 3)) & 1;
-          const uint8_t* marks = x.marks[32 * sub + k];
+          // the key's bit is with the lanes of its group
+          const uint32_t bits_of_group = (uint32_t)__shfl((int)seen, col + MR * (k / 4 % GL), 64);
+          const bool in = bits_of_group >> (k / KS * 4 + k % 4) & 1;
+          const uint8_t* bad = known.at[32 * sub + k];
 #pragma unroll
           for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int c = TYPE == KV_Q8 ? 0 : (32 * sub + k) * PR + 4 * d + q;
-              const uint32_t bits = TYPE == KV_Q8 ? marks[0] * 15u : x.bad[c % NT / 64] ? marks[4 * d + q] >> (4 * h) : 0u;
+            for (int q = 0; q < NQ; ++q) {
+              const int piece = (MR * d + KS * q + 4 * h) / 8, c = TYPE == KV_Q8 ? 0 : (32 * sub + k) * PR + piece;
+              const uint32_t bits = TYPE == KV_Q8 ? bad[0] * 15u : known.any[c % NT / 64] ? bad[piece] >> (4 * (h & 1)) : 0u;
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 if (in && (bits >> e & 1)) o[d][4 * q + e] = __uint_as_float(0x7fc00000u);
@@ -481,19 +547,32 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
 
   const bool busy = __any(valid);
   const int rounds = (tile1 - tile0 + NK - 1) / NK;
-  if (mine < k1) store_tile(mine, tiles[0]);
+  if (mine < k1) {
+    if (partly(mine)) mark(marks[kg][0]);
+    store_tile(tiles[0]);
+  }
   if constexpr (NR > 1) lds_barrier();
   for (int i = 0; i < rounds; ++i) {
-    const int t = mine + i * NK * TK, after = t + NK * TK;
+    const int t = mine + i * NK * TK, next = t + NK * TK < k1 ? t + NK * TK : t;  // the last turn stages its own again
     const Tile& x = tiles[NB == 2 ? i & 1 : 0];
-    if (after < k1) load_tile(after);
-    bool marked = false;
+    Tile& to = tiles[NB == 2 ? (i + 1) & 1 : 0];
+    const Marks& known = marks[kg][i & 1];
+    Marks& note = marks[kg][(i + 1) & 1];
+    if (busy && t < k1 && t < whi && t + TK > wlo) {
+      bool marked = false;
+      if (partly(t)) {
 #pragma unroll
-    for (int w = 0; w < (TYPE == KV_Q8 ? 1 : NR); ++w) marked |= __builtin_amdgcn_readfirstlane(x.bad[w]) != 0;
-    if (busy && t < k1 && t < whi && t + TK > wlo) compute(t, x, marked);
-    if (after < k1) store_tile(after, tiles[NB == 2 ? (i + 1) & 1 : 0]);
+        for (int w = 0; w < (TYPE == KV_Q8 ? 1 : NR); ++w) marked |= __builtin_amdgcn_readfirstlane(known.any[w]) != 0;
+      }
+      compute(t, x, known, marked, next, to, note);
+    } else if (t < k1) {
+      load_tile(next);
+      if (partly(next)) mark(note);
+      store_tile(to);
+    }
     if constexpr (NR > 1) lds_barrier();
   }
+  if constexpr (MR == 16) l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
 
   if constexpr (NK > 1) {
@@ -503,7 +582,7 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) g.o[kg - 1][rw][4 * d + q][lane] = f4_t{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+        for (int q = 0; q < NQ; ++q) g.o[kg - 1][rw][NQ * d + q][lane] = f4_t{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
       g.ml[kg - 1][rw][0][lane] = m, g.ml[kg - 1][rw][1][lane] = l;
       if (lane == 0) g.D[kg - 1][rw] = D;
     }
@@ -523,8 +602,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
 #pragma unroll
       for (int d = 0; d < ND; ++d)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const f4_t y = g.o[k][rw][4 * d + q][lane];
+        for (int q = 0; q < NQ; ++q) {
+          const f4_t y = g.o[k][rw][NQ * d + q][lane];
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[d][4 * q + e] += f * y[e];
         }
@@ -538,8 +617,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int at = 32 * d + 8 * q + 4 * h;
+      for (int q = 0; q < NQ; ++q) {
+        const int at = MR * d + KS * q + 4 * h;
         if (at < a.hd)
           *reinterpret_cast<f4u_t*>(out + at) = f4_t{o[d][4 * q] * inv, o[d][4 * q + 1] * inv, o[d][4 * q + 2] * inv, o[d][4 * q + 3] * inv};
       }
@@ -549,8 +628,8 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int at = 32 * d + 8 * q + 4 * h;
+      for (int q = 0; q < NQ; ++q) {
+        const int at = MR * d + KS * q + 4 * h;
         if (at < a.hd)
           *reinterpret_cast<f4_t*>(out + at) = f4_t{o[d][4 * q] * fo, o[d][4 * q + 1] * fo, o[d][4 * q + 2] * fo, o[d][4 * q + 3] * fo};
       }
@@ -558,25 +637,21 @@ __global__ void __launch_bounds__(256, HD == 256 ? 1 : 2) k_rows_attn(RowsAttnAr
   }
 }
 
-// Blocks on the device at a time, by their registers and LDS.
+// Blocks on the device at a time, by their LDS.
 int64_t full_of(const RowsAttnArgs& r, int nr) {
   const bool f32 = r.a.type == KV_F32;
-  const bool one = r.a.hd > 128 || (r.a.hd > 64 ? nr == 1 || (f32 && nr == 2) : f32 && nr == 1);
+  const bool one = r.a.hd > 128 ? nr < 4 || f32 : r.a.hd > 64 ? nr == 1 || (f32 && nr == 2) : f32 && nr == 1;
   return (int64_t)device_cus() * (one ? 1 : 2);
 }
 
-// Row waves of a block: as many as leave the device full (a tile is then staged once for more
-// rows), else the fewest that the type's tiles leave room for.
-int row_waves(const RowsAttnArgs& r) {
-  const int least = r.a.hd > 128 ? (r.a.type == KV_F32 ? 4 : 2) : r.a.type == KV_F32 && r.a.hd > 64 ? 2 : 1;
-  for (int nr = 4; nr > least; nr /= 2)
-    if ((r.R + 32 * nr - 1) / (32 * nr) * r.a.n_kv >= full_of(r, nr) * 3 / 4) return nr;
-  return least;
+int64_t row_blocks(const RowsAttnArgs& r, int nr) {
+  const int rows = row_tile(r.a.hd) * nr;
+  return (r.R + rows - 1) / rows * r.a.n_kv;
 }
 
 template <int TYPE, int HD, int NR>
 hipError_t go(const RowsAttnArgs& r, hipStream_t s) {
-  const int64_t blocks = (r.R + 32 * NR - 1) / (32 * NR) * r.a.n_kv * r.splits;
+  const int64_t blocks = row_blocks(r, NR) * r.splits;
   if (blocks > INT32_MAX) return hipErrorInvalidValue;
   UAII_LAUNCH((k_rows_attn<TYPE, HD, NR>), dim3((unsigned)blocks), dim3(256), 0, s, r);
   return hipGetLastError();
@@ -584,8 +659,8 @@ hipError_t go(const RowsAttnArgs& r, hipStream_t s) {
 
 template <int TYPE, int HD>
 hipError_t by_waves(const RowsAttnArgs& r, hipStream_t s) {
-  const int nr = row_waves(r);
-  if constexpr (HD == 64 || (HD == 128 && TYPE != KV_F32)) {
+  const int nr = r.nr;
+  if constexpr (HD == 64 || TYPE != KV_F32) {
     if (nr == 1) return go<TYPE, HD, 1>(r, s);
   }
   if constexpr (HD < 256 || TYPE != KV_F32) {
@@ -603,16 +678,44 @@ hipError_t by_width(const RowsAttnArgs& r, hipStream_t s) {
 
 }  // namespace
 
-// A split writes its rows' sums and the join reads them again, so there are splits only
-// where the blocks leave at least half the device idle, and of 128 keys at least.
-int rows_attn_splits(const RowsAttnArgs& r, int64_t keys) {
-  const int nr = row_waves(r);
-  const int64_t blocks = (r.R + 32 * nr - 1) / (32 * nr) * r.a.n_kv;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({128, (keys + 127) / 128, full_of(r, nr) / blocks}));
+// Row waves and key splits by an estimate of the launch's time, in cycles of a wave. Measured
+// on f16 caches of head_dim 128: a block's way to its first tile and from its last one 10 k; a
+// turn (32 keys) 3.5 k where each wave stages its own tiles, 2.8 k where two share one, 2.4 k
+// where four do (1.6 times the first two with rows of 256); 1.35 times that with two blocks
+// on a CU. A split writes its rows' sums and the
+// join reads them: 12 bytes a cycle and CU, and its own way. (4012 rows of 8 heads over a window of 1500, KV_Q8: two row
+// waves 73 us, four and two splits 88; 10400 rows of one head of 256 over 1300: four row waves
+// and three splits 42 us, two row waves 70.)
+void rows_attn_shape(RowsAttnArgs* r) {
+  const SeqAttnArgs& a = r->a;
+  int64_t most = a.n_prefix, mean = most;  // keys of a row
+  if (!r->prefix) {
+    most = std::max<int64_t>((int64_t)a.p0 + a.rows, a.bidir);
+    mean = std::max<int64_t>(a.p0 + (a.rows + 1) / 2, a.bidir);
+    if (a.window) most = std::min<int64_t>(most, (int64_t)a.window + row_tile(a.hd) * 4 / r->G), mean = std::min(mean, most);
+  }
+  const int least = a.type != KV_F32 ? 1 : a.hd > 128 ? 4 : a.hd > 64 ? 2 : 1;
+  const double row_bytes = (double)r->R * a.n_kv * part_stride(a.hd) * 8 / device_cus();
+  double best = 0;
+  for (int nr = 4; nr >= least; nr /= 2) {
+    const int nk = 4 / nr;
+    const int64_t blocks = row_blocks(*r, nr), full = full_of(*r, nr);
+    const double turn = (nr == 4 ? 2400 : nr == 2 ? 2800 : 3500) * (a.hd > 128 && nr < 4 ? 1.6 : a.hd > 64 ? 1.0 : 0.65) * (a.type == KV_F32 ? 1.5 : 1.0);
+    for (int64_t splits : {(int64_t)1, full / 2 / blocks, full / blocks}) {
+      splits = std::min<int64_t>({splits, 128, (most + 127) / 128});
+      if (splits < 1) continue;
+      const int64_t all = blocks * splits, waits = (all + full - 1) / full;
+      const double turns = std::max(1.0, (waits > 1 ? mean : most) / 32.0 / nk / splits);
+      const double shared = full > device_cus() && all > device_cus() ? 1.35 : 1.0;
+      double cost = (waits > 1 ? (double)all / full + 0.3 : 1.0) * (10e3 + turns * turn * shared);
+      if (splits > 1 || r->prefix) cost += splits * (row_bytes / 12 + 400) + 4e3;
+      if (best == 0 || cost < best) best = cost, r->nr = nr, r->splits = (int)splits;
+    }
+  }
 }
 
 hipError_t launch_rows_attn(const RowsAttnArgs& r, hipStream_t s) {
-  if (r.R <= 0 || r.splits < 1 || r.a.hd % 16 || r.a.hd < 16 || r.a.hd > 256 || ((r.splits > 1 || r.prefix) && !r.part))
+  if (r.R <= 0 || r.splits < 1 || (r.nr != 1 && r.nr != 2 && r.nr != 4) || r.a.hd % 16 || r.a.hd < 16 || r.a.hd > 256 || ((r.splits > 1 || r.prefix) && !r.part))
     return hipErrorInvalidValue;
   switch (r.a.type) {
     case KV_F32: return by_width<KV_F32>(r, s);

@@ -88,13 +88,13 @@ __device__ inline float weight_of(float m, float l, float M) {
 struct RowsAttnArgs {
   SeqAttnArgs a;
   int64_t R;      // rows of a kv head
-  int G, splits;  // key splits; with more than one, and for a prefix, partials are written
+  int G;
+  int nr, splits;  // row waves of a block and key splits (rows_attn_shape); with more than one split, and for a prefix, partials are written
   bool prefix;    // keys 0 .. n_prefix - 1 of kp, vp, for one query a sequence
   float* part;    // [splits][n_kv][R][part_stride]
 };
 
-// Key splits that fill the device (1: none needed).
-int rows_attn_splits(const RowsAttnArgs& r, int64_t keys);
+void rows_attn_shape(RowsAttnArgs* r);  // nr and splits from the rest
 hipError_t launch_rows_attn(const RowsAttnArgs& r, hipStream_t s);
 
 }  // namespace uaii_hip
