@@ -396,14 +396,17 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
       for (int k = 0; k < 4; ++k) s[4 * q + k] *= x[k];
     }
   };
-  // One tile, the next one's way to its place (`to`, `note`) beside it.
-  auto compute = [&](int t, const Tile& x, const Marks& known, bool marked, int next, Tile& to, Marks& note) __attribute__((always_inline)) {
+  // One tile, and beside it, where there is a `next` one, that one's way to its place (`to`, `note`).
+  auto compute = [&](auto more, int t, const Tile& x, const Marks& known, bool marked, int next, Tile& to, Marks& note) __attribute__((always_inline)) {
+    constexpr bool NEXT = decltype(more)::value;
 #pragma unroll
     for (int sub = 0; sub < SUBS; ++sub) {
       const int kt = t + 32 * sub, key0 = kt + 4 * h;
       float s[NE];
-      if (sub == 0) {
-        load_tile(next);
+      if constexpr (NEXT) {
+        if (sub == 0) load_tile(next);
+      }
+      if (NEXT && sub == 0) {
         products(x, sub, s, std::integral_constant<int, 2 * PIECES * PW + (TYPE == KV_Q8)>{});
       } else {
         products(x, sub, s, std::integral_constant<int, 0>{});
@@ -472,7 +475,9 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
           for (int d = 0; d < ND; ++d) o[d] *= beta;
         }
       }
-      if (sub + 1 == SUBS && partly(next)) mark(note);
+      if constexpr (NEXT) {
+        if (sub + 1 == SUBS && partly(next)) mark(note);
+      }
       const float ref = (m == -INFINITY ? 0.0f : m) + lgD - 10.0f;
       f4_t sum = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -508,7 +513,9 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
           if constexpr (PL == 2) o[d] = mfma(v_at(1, c, d), phi, o[d]);
         }
       }
-      if (sub + 1 == SUBS) store_tile(to);
+      if constexpr (NEXT) {
+        if (sub + 1 == SUBS) store_tile(to);
+      }
       {
         constexpr int OPS = PL == 2 ? 3 : 2, READS = 2 * PL, STEPS = NE / 8 * ND, AHEAD = STEPS > 4 ? 3 : 2;
         constexpr int WRITES = (2 * PIECES * (TYPE == KV_F16 ? 1 : 2) + (TYPE == KV_Q8) + AHEAD - 1) / AHEAD;
@@ -521,7 +528,7 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
           __builtin_amdgcn_sched_group_barrier(0x8, OPS, 1);
-          if (sub + 1 == SUBS) __builtin_amdgcn_sched_group_barrier(0x200, WRITES, 1);
+          if (NEXT && sub + 1 == SUBS) __builtin_amdgcn_sched_group_barrier(0x200, WRITES, 1);
         }
       }
       if (marked) {  // rows that see a value that is not finite
@@ -552,25 +559,34 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
     store_tile(tiles[0]);
   }
   if constexpr (NR > 1) lds_barrier();
-  for (int i = 0; i < rounds; ++i) {
-    const int t = mine + i * NK * TK, next = t + NK * TK < k1 ? t + NK * TK : t;  // the last turn stages its own again
-    const Tile& x = tiles[NB == 2 ? i & 1 : 0];
-    Tile& to = tiles[NB == 2 ? (i + 1) & 1 : 0];
-    const Marks& known = marks[kg][i & 1];
-    Marks& note = marks[kg][(i + 1) & 1];
-    if (busy && t < k1 && t < whi && t + TK > wlo) {
-      bool marked = false;
-      if (partly(t)) {
+  auto marked = [&](int t, const Marks& known) __attribute__((always_inline)) {
+    bool any = false;
+    if (partly(t)) {
 #pragma unroll
-        for (int w = 0; w < (TYPE == KV_Q8 ? 1 : NR); ++w) marked |= __builtin_amdgcn_readfirstlane(known.any[w]) != 0;
-      }
-      compute(t, x, known, marked, next, to, note);
-    } else if (t < k1) {
+      for (int w = 0; w < (TYPE == KV_Q8 ? 1 : NR); ++w) any |= __builtin_amdgcn_readfirstlane(known.any[w]) != 0;
+    }
+    return any;
+  };
+  // a tile that the wave's rows meet
+  auto met = [&](int t) __attribute__((always_inline)) { return busy && t < whi && t + TK > wlo; };
+  int t = mine;
+  for (int i = 0; i + 1 < rounds; ++i) {  // a group that has no tile in the last round stages this one again
+    const int next = t + NK * TK < k1 ? t + NK * TK : t;
+    Tile& to = tiles[NB == 2 ? (i + 1) & 1 : 0];
+    Marks& note = marks[kg][(i + 1) & 1];
+    if (met(t)) {
+      compute(std::true_type{}, t, tiles[NB == 2 ? i & 1 : 0], marks[kg][i & 1], marked(t, marks[kg][i & 1]), next, to, note);
+    } else {
       load_tile(next);
       if (partly(next)) mark(note);
       store_tile(to);
     }
+    t += NK * TK;
     if constexpr (NR > 1) lds_barrier();
+  }
+  if (rounds > 0 && t < k1 && met(t)) {
+    const int i = rounds - 1;
+    compute(std::false_type{}, t, tiles[NB == 2 ? i & 1 : 0], marks[kg][i & 1], marked(t, marks[kg][i & 1]), t, tiles[0], marks[kg][0]);
   }
   if constexpr (MR == 16) l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
