@@ -23,7 +23,7 @@ struct BatchArgs {
   int G, groups;       // query heads of a kv head, and its row groups of RC
   float* slots;        // [2 blocks][RC][part_stride]: a block's first and last run
   float* whole;        // [n_seq * n_kv * groups][RC][part_stride], with a prefix only
-  int* info;           // first unit of each (sequence, kv head, group), then the units of all
+  int2* info;          // for each (sequence, kv head, group): its first block, and how many follow
   const float* pre;    // partials over the prefix (RowsAttnArgs::part)
   int pre_splits, blocks;
   int parts;           // > 0: a block for each of so many units of every head, used or not
@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
 
   // ---- this block's units [u, u1) of the batch's, and the sequence that holds the first
   int s, base, u, u1;  // base: the first unit of sequence s
+  int total = 0, blocks = 0;
   if (b.parts > 0) {
     // few units in all: block by block, and those behind a head's last one have nothing to do
     const int hx = (int)blockIdx.x / b.parts, uu = (int)blockIdx.x % b.parts;
@@ -105,7 +106,6 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
     u = hx % H * n + uu;
     u1 = u + 1;
   } else {
-    int total;
     if (n_seq <= 64) {
       // a lane for each sequence, in every wave
       const int n = lane < n_seq ? span_of(a, lane).units() : 0;
@@ -154,8 +154,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
       __syncthreads();
       s = __builtin_amdgcn_readfirstlane(found[0]), base = __builtin_amdgcn_readfirstlane(found[1]) * H;
     }
-    if (blockIdx.x == 0 && tid == 0) b.info[(int64_t)n_seq * H] = total;
-    const int blocks = min(b.blocks, total);  // each has a unit at least
+    blocks = min(b.blocks, total);  // each has a unit at least
     if ((int)blockIdx.x >= blocks) return;
     u = (int)((int64_t)total * blockIdx.x / blocks);
     u1 = (int)((int64_t)total * (blockIdx.x + 1) / blocks);
@@ -177,7 +176,6 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
     const int kvh = hx / b.groups, head0 = kvh * b.G + hx % b.groups * RC;
     const int rows = min(RC, b.G - hx % b.groups * RC);
     const int k0 = sp.lo + UNIT * uu, k1 = min(sp.n, sp.lo + UNIT * ue);
-    if (b.parts == 0 && uu == 0 && tid == 0) b.info[(int64_t)s * H + hx] = u;
 
     const int64_t first = (int64_t)kvh * a.max_seq;
     const uint8_t* kbase = a.kc + (int64_t)s * a.seq_bytes;
@@ -476,6 +474,11 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
     }
     __syncthreads();
     const bool complete = uu == 0 && ue == units;
+    if (b.parts == 0 && uu == 0 && tid == 0) {
+      // block of unit v: the last one whose first unit, total b / blocks, is not behind it
+      const int last = complete ? (int)blockIdx.x : (int)(((int64_t)(u + units) * blocks - 1) / total);
+      b.info[(int64_t)s * H + hx] = make_int2((int)blockIdx.x, last - (int)blockIdx.x);
+    }
     const int64_t stride = part_stride(a.hd);
     const bool direct = complete && b.pre_splits == 0;
     float* part = b.parts > 0 ? b.slots + (int64_t)blockIdx.x * RC * stride
@@ -515,10 +518,11 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
 // eight partials of a wave at a time.
 struct JoinArgs {
   SeqAttnArgs a;
-  int G, rc, groups, blocks, parts;
+  int G, rc, groups, parts;
   const float* slots;
   const float* whole;
-  const int* info;       // null: no own keys (prompt rows)
+  const int2* info;      // with parts 0
+  bool batch;            // rows have own keys
   const float* part;     // [splits][n_kv][rows * G][part_stride]
   int splits;
 };
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(64 * W) k_attn_join(JoinArgs j) {
   int own = 0;
   int64_t ahead = 0, step = 0;  // floats from the first to the second, and from there on
   const float* at = nullptr;
-  if (j.info) {
+  if (j.batch) {
     const Span sp = span_of(a, row);
     const int units = sp.units();
     if (units > 0) {
@@ -547,13 +551,10 @@ __global__ void __launch_bounds__(64 * W) k_attn_join(JoinArgs j) {
         at = j.slots + ((int64_t)row * H + hx) * j.parts * j.rc * stride;
         ahead = step = j.rc * stride;
       } else {
-        const int64_t first = j.info[(int64_t)row * H + hx], total = j.info[a.rows * H];
-        // block of unit u: the last one whose first unit, total b / blocks, is not behind it
-        const int64_t blocks = min((int64_t)j.blocks, total);
-        const int b0 = (int)(((first + 1) * blocks - 1) / total);
-        own = (int)(((first + units) * blocks - 1) / total) - b0 + 1;
-        at = own == 1 ? j.whole + ((int64_t)row * H + hx) * j.rc * stride : j.slots + (2 * (int64_t)b0 + 1) * j.rc * stride;
-        ahead = j.rc * stride, step = 2 * ahead;  // the last run of block b0, the first runs of those behind it
+        const int2 at_blocks = j.info[(int64_t)row * H + hx];
+        own = at_blocks.y + 1;
+        at = own == 1 ? j.whole + ((int64_t)row * H + hx) * j.rc * stride : j.slots + (2 * (int64_t)at_blocks.x + 1) * j.rc * stride;
+        ahead = j.rc * stride, step = 2 * ahead;  // the last run of the first block, the first runs of those behind it
       }
       if (own == 1 && j.splits == 0) return;  // written
       at += gr % j.rc * stride;
@@ -672,7 +673,7 @@ Plan plan_of(const SeqAttnArgs& a) {
     p.parts = heads * parts <= 2 * resident ? (int)parts : 0;
     p.blocks = (int)std::min<int64_t>(heads * parts, p.parts ? 2 * resident : resident);
     p.slots = pad256((p.parts ? 1 : 2) * (size_t)p.blocks * p.rc * row);
-    p.info = p.parts ? 0 : pad256(((size_t)heads + 1) * 4);
+    p.info = p.parts ? 0 : pad256((size_t)heads * sizeof(int2));
     if (a.n_prefix > 0) {
       p.rows.prefix = true;
       rows_attn_shape(&p.rows);
@@ -709,7 +710,7 @@ hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
     b.groups = p.groups;
     b.slots = reinterpret_cast<float*>(scratch + p.part);
     b.whole = reinterpret_cast<float*>(scratch + p.part + p.slots);
-    b.info = reinterpret_cast<int*>(scratch + p.part + p.slots + p.whole);
+    b.info = reinterpret_cast<int2*>(scratch + p.part + p.slots + p.whole);
     b.pre = j.part;
     b.pre_splits = p.splits;
     b.blocks = p.blocks;
@@ -721,11 +722,11 @@ hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
     if (e != hipSuccess) return e;
     j.rc = p.rc;
     j.groups = p.groups;
-    j.blocks = p.blocks;
     j.parts = p.parts;
     j.slots = b.slots;
     j.whole = b.whole;
     j.info = b.info;
+    j.batch = true;
   }
   // about how many partials a row has: a wave takes eight in one round trip
   const int64_t parts = p.splits + (a.n_keys ? std::max<int64_t>(1, p.blocks / (a.rows * a.n_kv * p.groups)) : 0);
