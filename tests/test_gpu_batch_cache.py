@@ -285,6 +285,28 @@ def test_batch_prefix(hip, t, prefix, shape):
     check_batch(hip, np.random.default_rng(3), t, *shape, lens=[5, 0, 200, 1, 33], seq=200, prefix=prefix)
 
 
+# (shape, sequences, prefix): too much for each sequence to read the prefix by itself, with few
+# and many query rows, a last row tile of one row, prefixes of whole tiles and not
+SHARED = [((8, 2, 64), 50, 2100), ((32, 8, 128), 20, 1300), ((5, 1, 80), 70, 3000), ((4, 2, 256), 40, 2600), ((14, 2, 32), 36, 2816),
+          ((8, 8, 64), 3, 8500), ((8, 8, 128), 33, 800), ((4, 1, 256), 65, 3100), ((20, 4, 112), 13, 4001)]
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape,n,prefix", SHARED, ids=str)
+def test_batch_shared_prefix(hip, t, shape, n, prefix):
+    assert n * prefix * shape[1] > 192 << 10
+    check_batch(hip, np.random.default_rng(3), t, *shape, lens=[(7 * i) % 45 for i in range(n)], seq=45, prefix=prefix)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape,n,prefix", SHARED[:2] + SHARED[3:4], ids=str)
+@pytest.mark.parametrize("opt", [dict(cap=30.0), dict(slopes=True), dict(window=20), dict(window=700), dict(window=1000, cap=4.0, slopes=True, spread=4.0)],
+                         ids=str)
+def test_batch_shared_prefix_options(hip, t, shape, n, prefix, opt):
+    """A window may hide all of the prefix from some sequences, a part of it from others."""
+    check_batch(hip, np.random.default_rng(5), t, *shape, lens=[(7 * i) % 45 for i in range(n)], seq=45, prefix=prefix, **opt)
+
+
 @pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
 @pytest.mark.parametrize("prefix", [0, 200])
 @pytest.mark.parametrize("opt", [dict(cap=30.0), dict(cap=0.5), dict(slopes=True), dict(window=1), dict(window=50), dict(window=150),

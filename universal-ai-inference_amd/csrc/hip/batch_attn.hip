@@ -26,6 +26,7 @@ struct BatchArgs {
   int2* info;          // for each (sequence, kv head, group): its first block, and how many follow
   const float* pre;    // partials over the prefix (RowsAttnArgs::part)
   int pre_splits, blocks;
+  int fold;            // keys of a prefix that each sequence reads with its own
   int parts;           // > 0: a block for each of so many units of every head, used or not
 };
 
@@ -33,15 +34,22 @@ __device__ inline f4_t mfma32(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_
 __device__ inline f4_t mfma16(h4_t a, h4_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
 __device__ inline f4_t mfma4(float a, float b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
+// What a sequence reads: with a prefix that is read with it (`fold` keys), the visible ones of
+// that, padded to whole tiles, and behind them its own. Both are one run of places:
+// 0 .. pre - 1 are prefix keys plo + place, padded .. end - 1 its own keys lo + place - padded.
 struct Span {
-  int n, lo;  // keys lo .. n - 1 of the sequence
-  __device__ int units() const { return (n - lo + UNIT - 1) / UNIT; }
+  int plo, pre, padded, lo, end;
+  __device__ int units() const { return (end + UNIT - 1) / UNIT; }
 };
 
-__device__ inline Span span_of(const SeqAttnArgs& a, int64_t s) {
+__device__ inline Span span_of(const SeqAttnArgs& a, int fold, int64_t s) {
   Span p;
-  p.n = (int)min((int64_t)max(a.n_keys[s], 0), a.max_seq);
-  p.lo = a.window ? max(0, p.n - a.window) : 0;
+  const int n = (int)min((int64_t)max(a.n_keys[s], 0), a.max_seq);
+  p.lo = a.window ? max(0, n - a.window) : 0;
+  p.plo = a.window ? min(fold, max(0, fold + n - a.window)) : 0;
+  p.pre = fold - p.plo;
+  p.padded = (p.pre + 31) & ~31;
+  p.end = p.padded + n - p.lo;
   return p;
 }
 
@@ -100,7 +108,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
     // few units in all: block by block, and those behind a head's last one have nothing to do
     const int hx = (int)blockIdx.x / b.parts, uu = (int)blockIdx.x % b.parts;
     s = hx / H;
-    const int n = span_of(a, s).units();
+    const int n = span_of(a, b.fold, s).units();
     if (uu >= n) return;
     base = 0;
     u = hx % H * n + uu;
@@ -108,7 +116,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
   } else {
     if (n_seq <= 64) {
       // a lane for each sequence, in every wave
-      const int n = lane < n_seq ? span_of(a, lane).units() : 0;
+      const int n = lane < n_seq ? span_of(a, b.fold, lane).units() : 0;
       int incl = n;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -122,7 +130,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
     } else {
       const int per = (n_seq + 255) / 256, s0 = min(n_seq, tid * per), s1 = min(n_seq, s0 + per);
       int mine = 0;
-      for (int i = s0; i < s1; ++i) mine += span_of(a, i).units();
+      for (int i = s0; i < s1; ++i) mine += span_of(a, b.fold, i).units();
       int incl = mine;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
@@ -144,7 +152,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
       if (before * H <= at && at < (before + mine) * H) {
         int i = s0;
         for (;; ++i) {
-          const int n = span_of(a, i).units();
+          const int n = span_of(a, b.fold, i).units();
           if (at < (before + n) * H) break;
           before += n;
         }
@@ -165,34 +173,43 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
   const bool low = PACK && col >= 8;      // it works on the low halves
 
   while (u < u1) {
-    Span sp = span_of(a, s);
+    Span sp = span_of(a, b.fold, s);
     int units = sp.units();
     while (units == 0) {  // sequences with no keys
       if (++s >= n_seq) return;
-      sp = span_of(a, s);
+      sp = span_of(a, b.fold, s);
       units = sp.units();
     }
     const int hx = (u - base) / units, uu = (u - base) % units, ue = min(units, uu + u1 - u);
     const int kvh = hx / b.groups, head0 = kvh * b.G + hx % b.groups * RC;
     const int rows = min(RC, b.G - hx % b.groups * RC);
-    const int k0 = sp.lo + UNIT * uu, k1 = min(sp.n, sp.lo + UNIT * ue);
+    const int k0 = UNIT * uu, k1 = min(sp.end, UNIT * ue);  // places
 
-    const int64_t first = (int64_t)kvh * a.max_seq;
-    const uint8_t* kbase = a.kc + (int64_t)s * a.seq_bytes;
-    const uint8_t* vbase = a.vc + (int64_t)s * a.seq_bytes;
-    const float* kscale = reinterpret_cast<const float*>(kbase + (int64_t)a.n_kv * a.max_seq * a.hd) + first;  // KV_Q8
-    const float* vscale = reinterpret_cast<const float*>(vbase + (int64_t)a.n_kv * a.max_seq * a.hd) + first;
-    kbase += first * a.hd * ES;
-    vbase += first * a.hd * ES;
+    // the sources: the prefix's cache and the sequence's, from the kv head's first row on, so
+    // that a place's row is the place in both
+    struct Source {
+      const uint8_t *k, *v;
+      const float *kscale, *vscale;  // KV_Q8
+    };
+    const uint32_t row_bytes = (uint32_t)a.hd * ES;
+    auto source = [&](const uint8_t* k, const uint8_t* v, int64_t seq, int64_t first) __attribute__((always_inline)) {
+      const int64_t row = kvh * seq + first, scales = (int64_t)a.n_kv * seq * a.hd;
+      return Source{k + row * row_bytes, v + row * row_bytes, reinterpret_cast<const float*>(k + scales) + row,
+                    reinterpret_cast<const float*>(v + scales) + row};
+    };
+    const Source shared = source(a.kp, a.vp, a.pre_seq, sp.plo);
+    const Source own = source(a.kc + (int64_t)s * a.seq_bytes, a.vc + (int64_t)s * a.seq_bytes, a.max_seq, (int64_t)sp.lo - sp.padded);
+    // places of tile t's source that are keys end here
+    auto limit = [&](int t) __attribute__((always_inline)) { return t < sp.padded ? min(sp.pre, k1) : k1; };
 
     uint32_t kw[NS][KW], vw[NS][4][VW];  // a tile: the lane's parts of its keys and of its values
     float fw;                            // KV_Q8: a key's factor in the lower lanes, a value's in the upper
     // keys behind the last repeat it and are masked; dims behind the row's end repeat its
     // last piece, which meets zeros of q or goes to outputs that are not stored
-    const uint32_t row_bytes = (uint32_t)a.hd * ES;
     auto load_keys = [&](int t) __attribute__((always_inline)) {
-      const gptr_t kt = uniform_at(kbase, (int64_t)t * row_bytes);
-      const int last = __builtin_amdgcn_readfirstlane(k1 - 1 - t);
+      const bool pre = t < sp.padded;
+      const int from = min(t, limit(t) - 1), last = limit(t) - 1 - from;  // a tile of padding repeats the last key too
+      const gptr_t kt = uniform_at(pre ? shared.k : own.k, (int64_t)from * row_bytes);
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const uint32_t kr = (uint32_t)min(16 * i + col, last) * row_bytes;
@@ -203,11 +220,15 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
           kw[i][w] = y[0], kw[i][w + 1] = y[1], kw[i][w + 2] = y[2], kw[i][w + 3] = y[3];
         }
       }
-      if constexpr (SC) fw = (lane < 32 ? kscale : vscale)[t + min(lane & 31, last)];
+      if constexpr (SC) {
+        const float* kf = pre ? shared.kscale : own.kscale;
+        const float* vf = pre ? shared.vscale : own.vscale;
+        fw = (lane < 32 ? kf : vf)[from + min(lane & 31, last)];
+      }
     };
     auto load_values = [&](int t) __attribute__((always_inline)) {
-      const gptr_t vt = uniform_at(vbase, (int64_t)t * row_bytes);
-      const int last = __builtin_amdgcn_readfirstlane(k1 - 1 - t);
+      const int from = min(t, limit(t) - 1), last = limit(t) - 1 - from;
+      const gptr_t vt = uniform_at(t < sp.padded ? shared.v : own.v, (int64_t)from * row_bytes);
       const uint32_t d = (uint32_t)min(col * E, a.hd - E) * ES;
 #pragma unroll
       for (int i = 0; i < NS; ++i)
@@ -346,15 +367,15 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
       }
       float y_of = mul;
       if (capped) {
-        float far = 0.0f;
+        float out = 0.0f;
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             y[i][r] *= to_cap;
-            far = fmaxf(far, fabsf(y[i][r]));
+            out = fmaxf(out, fabsf(y[i][r]));
           }
-        const bool some_far = __any(!(far < kTanhNear));
+        const bool some_far = __any(!(out < kTanhNear));
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
@@ -364,17 +385,19 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
           }
       }
       if (sloped) {
+        // positions between the tile's first key and the query (own keys: the query is the last of them)
+        const int far = sp.end - 1 - t + (t < sp.padded ? sp.pre - sp.padded + sp.lo : 0);
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[i][r] = fmaf(y[i][r], mul, -slope * (float)(sp.n - 1 - (t + 16 * i + 4 * g + r)));
+          for (int r = 0; r < 4; ++r) y[i][r] = fmaf(y[i][r], mul, -slope * (float)(far - 16 * i - 4 * g - r));
         y_of = 1.0f;
       }
-      if (t + KT > k1) {
+      if (t + KT > limit(t)) {
 #pragma unroll
         for (int i = 0; i < NS; ++i)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[i][r] = t + 16 * i + 4 * g + r < k1 ? y[i][r] : -INFINITY;
+          for (int r = 0; r < 4; ++r) y[i][r] = t + 16 * i + 4 * g + r < limit(t) ? y[i][r] : -INFINITY;
       }
       float top = -INFINITY;
 #pragma unroll
@@ -518,7 +541,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
 // eight partials of a wave at a time.
 struct JoinArgs {
   SeqAttnArgs a;
-  int G, rc, groups, parts;
+  int G, rc, groups, parts, fold;
   const float* slots;
   const float* whole;
   const int2* info;      // with parts 0
@@ -542,7 +565,7 @@ __global__ void __launch_bounds__(64 * W) k_attn_join(JoinArgs j) {
   int64_t ahead = 0, step = 0;  // floats from the first to the second, and from there on
   const float* at = nullptr;
   if (j.batch) {
-    const Span sp = span_of(a, row);
+    const Span sp = span_of(a, j.fold, row);
     const int units = sp.units();
     if (units > 0) {
       const int hx = kvh * j.groups + gr / j.rc;
@@ -645,12 +668,23 @@ int resident_blocks(int type, int hd, bool pack) {
 }
 
 struct Plan {
-  int G, groups, rc, blocks, parts, splits;
+  int G, groups, rc, blocks, parts, splits, fold;
   bool pack;
   RowsAttnArgs rows;
   size_t part, slots, whole, info;  // bytes of the scratch's parts
   size_t bytes() const { return part + slots + whole + info; }
 };
+
+// Whether each sequence reads the prefix with its own keys, where that is little: a launch and
+// its partials are saved, and the reads after the first come from caches. Measured, read with
+// each sequence against once for all (us): f16, 8 heads of 128, 4 sequences over 100 keys 9.9,
+// 16.9, 32 over 500 (62 MB, 128 k keys of heads) 21.5, 22.0, 8 over 6000 (187 MB) 24.9, 22.7,
+// 48 over 2000 47.6, 35.4; KV_Q8, 4 heads of 64, 8 over 6000 (192 k keys) 19.8, 19.7, 5 over
+// 30011 28.1, 22.6.
+bool folds(const SeqAttnArgs& a) {
+  const int64_t keys = a.rows * a.n_prefix;
+  return a.n_prefix > 0 && keys * a.n_kv <= 192 << 10 && keys * kv_seq_bytes(a.type, a.n_kv, 1, a.hd) * 2 <= (int64_t)64 << 20;
+}
 
 size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
 
@@ -668,13 +702,15 @@ Plan plan_of(const SeqAttnArgs& a) {
     p.pack = a.type != KV_F32 && p.G <= 8;
     p.rc = rows_of(p.pack);
     p.groups = (p.G + p.rc - 1) / p.rc;
-    const int64_t heads = a.rows * a.n_kv * p.groups, held = a.window ? std::min<int64_t>(a.window, a.max_seq) : a.max_seq;
+    p.fold = folds(a) ? a.n_prefix : 0;
+    const int64_t heads = a.rows * a.n_kv * p.groups;
+    const int64_t held = (a.window ? std::min<int64_t>(a.window, a.max_seq + p.fold) : a.max_seq + p.fold) + (p.fold ? 31 : 0);
     const int64_t parts = (held + UNIT - 1) / UNIT, resident = resident_blocks(a.type, a.hd, p.pack);
     p.parts = heads * parts <= 2 * resident ? (int)parts : 0;
     p.blocks = (int)std::min<int64_t>(heads * parts, p.parts ? 2 * resident : resident);
     p.slots = pad256((p.parts ? 1 : 2) * (size_t)p.blocks * p.rc * row);
     p.info = p.parts ? 0 : pad256((size_t)heads * sizeof(int2));
-    if (a.n_prefix > 0) {
+    if (a.n_prefix > p.fold) {
       p.rows.prefix = true;
       rows_attn_shape(&p.rows);
       p.splits = p.rows.splits;
@@ -715,6 +751,7 @@ hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
     b.pre_splits = p.splits;
     b.blocks = p.blocks;
     b.parts = p.parts;
+    b.fold = p.fold;
     e = with_kernel(a.type, a.hd, p.pack, [&](auto kernel) {
       UAII_LAUNCH(kernel, dim3((unsigned)b.blocks), dim3(256), 0, s, b);
       return hipGetLastError();
@@ -723,6 +760,7 @@ hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
     j.rc = p.rc;
     j.groups = p.groups;
     j.parts = p.parts;
+    j.fold = p.fold;
     j.slots = b.slots;
     j.whole = b.whole;
     j.info = b.info;

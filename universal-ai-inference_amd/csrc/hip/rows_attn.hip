@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
       if constexpr (SC) {
         const float f = x.vf[32 * sub + (lane & 31)];
         if (__any(f > D && f < INFINITY)) {
-          const float big = wave_max(f < INFINITY ? f : 0.0f);
+          const float big = wave_max_dpp(f < INFINITY ? f : 0.0f);
           const int e = min(126, (int)((__float_as_uint(big) >> 23) & 0xff) - 126);  // the next power of two
           const float Dnew = pow2i(e), beta = D / Dnew;
           D = Dnew;
