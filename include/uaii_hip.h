@@ -220,10 +220,14 @@ UAII_HIP_API int uaii_hip_attention_prefill(const float* q, const void* kcache,
  * head-major, [n_kv_heads][max_seq][head_dim], the layout of the entry points above; an
  * UAII_HIP_KV_Q8 cache holds bytes there and, behind them, [n_kv_heads][max_seq] f32
  * scales: a value is (byte - 128) * scale, a head's row having one scale, max |x| / 127
- * (the next lower number where 127 of it would pass the end of f32). Rows with an infinity or a NaN read back as NaN. A batch's caches lie one behind the
- * other, sequence s at s * uaii_hip_kv_cache_bytes. Caches are 16-byte aligned; head_dim
- * is a multiple of 16 up to 256; max_seq, and a prefix and max_seq together, are at most 2^30
- * positions. */
+ * (the next lower number where 127 of it would pass the end of f32). Rows with an infinity
+ * or a NaN read back as NaN. A batch's caches lie one behind the other, sequence s at
+ * s * uaii_hip_kv_cache_bytes. Caches are 16-byte aligned; head_dim is a multiple of 16 up
+ * to 256; max_seq, and a prefix and max_seq together, are at most 2^30 positions.
+ *
+ * The attentions take any bytes in places that a query does not see. A key that it sees and
+ * that is not finite makes its result NaN or not finite, such a value that dimension of the
+ * result (all of them with UAII_HIP_KV_Q8). */
 #define UAII_HIP_KV_F32 0
 #define UAII_HIP_KV_F16 1
 #define UAII_HIP_KV_Q8 2
@@ -248,7 +252,7 @@ UAII_HIP_API int uaii_hip_kv_read(const void* cache, int kv_type, int64_t n_seq,
 typedef struct uaii_hip_score_options {
   uint32_t struct_size;
   float scale;         /* 0: 1 / sqrt(head_dim) */
-  float softcap;       /* 0: none */
+  float softcap;       /* 0: none; at most 1e20 */
   const float* slopes; /* device, one for each query head; NULL: none */
   int64_t window;      /* > 0: keys at i - window + 1 and after only; 0: all */
 } uaii_hip_score_options;
@@ -259,7 +263,8 @@ UAII_HIP_API void uaii_hip_score_options_init(uaii_hip_score_options* options);
  * over the sequence's own n_keys[s] keys, at positions n_prefix + j. The query is at the
  * last of these positions. n_keys is a device array; a length outside 0 .. max_seq counts as
  * the nearer of the two. A query that sees no key gets zeros. options may be NULL.
- * q and out must not overlap. Its scratch is the library's (see uaii_hip_gemm). */
+ * q and out must not overlap (rows of one pitch may lie between each other). Its scratch is
+ * the library's (see uaii_hip_gemm). */
 UAII_HIP_API int uaii_hip_attention_batch(const float* q, int64_t ldq, int64_t n_seq, const void* kcache,
                                           const void* vcache, int kv_type, int64_t max_seq, const int32_t* n_keys,
                                           const void* kprefix, const void* vprefix, int64_t prefix_seq,
@@ -271,7 +276,7 @@ UAII_HIP_API int uaii_hip_attention_batch(const float* q, int64_t ldq, int64_t n
  * j < bidirectional (0: causal; at most p0 + m); of these only j >= first_key[i - p0], where
  * that device array of m is given (packed documents; padding sees nothing behind its own
  * position), and those in the options' window. A query that sees no key gets zeros.
- * q and out must not overlap. */
+ * q, out and scratch as for uaii_hip_attention_batch. */
 UAII_HIP_API int uaii_hip_attention_prompt(const float* q, int64_t ldq, int64_t m, const void* kcache,
                                            const void* vcache, int kv_type, int64_t max_seq, int64_t p0,
                                            int64_t bidirectional, const int32_t* first_key, int n_heads,

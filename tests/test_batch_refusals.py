@@ -112,3 +112,16 @@ def test_options_init():
     o = ScoreOptions(scale=3.0, softcap=2.0, window=9)
     uaii_amd.lib().uaii_hip_score_options_init(ctypes.byref(o))
     assert (o.struct_size, o.scale, o.softcap, o.slopes, o.window) == (ctypes.sizeof(ScoreOptions), 0.0, 0.0, None, 0)
+
+
+@pytest.mark.parametrize("batch", [True, False])
+def test_softcap_has_an_end(batch):
+    assert attn_call(batch, opt=dict(softcap=1.01e20)) == REFUSED
+
+
+@pytest.mark.parametrize("batch", [True, False])
+@pytest.mark.parametrize("bad", [dict(out=A + 4 * 2047, ldq=4096, ldo=4096), dict(out=A + 4 * 2049, ldq=4096, ldo=4096),
+                                 dict(out=A + 4 * 2048, ldq=4096, ldo=4097), dict(out=A + 4 * 4096, ldq=4096, ldo=4096)], ids=str)
+def test_rows_that_meet(batch, bad):
+    """Rows of one pitch may lie between each other, if none touches another; with two pitches the ranges count."""
+    assert attn_call(batch, **bad) == REFUSED

@@ -370,6 +370,58 @@ def test_batch_value_not_finite(hip, t, prefix):
     assert np.isfinite(got[0]).all() and np.isfinite(got[2]).all() and np.isfinite(got[1, 2:]).all()
 
 
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("cap", [1e-38, 1e-20, 1e20])
+def test_extreme_softcap(hip, t, cap):
+    """A cap that makes all scores alike, those of a query of zeros too, and one that changes none."""
+    rng = np.random.default_rng(10)
+    heads, kv, hd, seq = 4, 2, 64, 70
+    k, v, q = rows(rng, 1, kv, seq, hd), rows(rng, 1, kv, seq, hd), rows(rng, 2, heads * hd)
+    q[1] = 0.0
+    (kc, kx), (vc, vx) = pack(k, t), pack(v, t)
+    twice = lambda c: torch.cat([c, c])  # noqa: E731
+    dq, dn, opt = torch.from_numpy(q).cuda(), torch.tensor([seq, seq - 1], dtype=torch.int32, device="cuda"), options(cap)
+    kc2, vc2, out = twice(kc), twice(vc), torch.zeros(2, 2, heads * hd, device="cuda")
+    check_hip(hip.uaii_hip_attention_batch(ptr(dq), I64(heads * hd), I64(2), ptr(kc2), ptr(vc2), t, I64(seq), ptr(dn), None, None, I64(0),
+                                           I64(0), heads, kv, hd, ctypes.byref(opt), ptr(out[0]), I64(heads * hd), None))
+    check_hip(hip.uaii_hip_attention_prompt(ptr(dq), I64(heads * hd), I64(2), ptr(kc), ptr(vc), t, I64(seq), I64(seq - 2), I64(0), None, heads,
+                                            kv, hd, ctypes.byref(opt), ptr(out[1]), I64(heads * hd), None))
+    got, at, none = out.cpu().numpy(), np.arange(seq), np.zeros(2)
+    for h in range(heads):
+        for call, hi in ((0, [seq, seq - 1]), (1, [seq - 1, seq])):
+            w, tol = attend(q[:, h * hd : (h + 1) * hd], kx[0, h // 2], vx[0, h // 2], at, none, none, np.array(hi), 0.125, float(np.float32(cap)), 0.0)
+            if cap == 1e20:  # its 8 u of a cap, in the bound, are 8 u of the scores here: cap tanh(s / cap) is s
+                w, tol = attend(q[:, h * hd : (h + 1) * hd], kx[0, h // 2], vx[0, h // 2], at, none, none, np.array(hi), 0.125, 0.0, 0.0)
+                tol = 2 * tol
+            close(got[call][:, h * hd : (h + 1) * hd], w, tol)
+
+
+@pytest.mark.parametrize("batch", [False, True])
+def test_rows_between_each_other(hip, batch):
+    """q and out as columns of one buffer."""
+    rng = np.random.default_rng(11)
+    heads, kv, hd, seq, n = 4, 2, 64, 50, 3
+    k, v, q = rows(rng, n, kv, seq, hd), rows(rng, n, kv, seq, hd), rows(rng, n, heads * hd)
+    (kc, kx), (vc, vx) = pack(k, KV_F16), pack(v, KV_F16)
+    width = heads * hd
+    both = torch.full((n, 2 * width + 4), -7.0, device="cuda")
+    both[:, :width] = torch.from_numpy(q).cuda()
+    lens, out, ld = torch.tensor([50, 7, 20], dtype=torch.int32, device="cuda"), both[:, width:], I64(2 * width + 4)
+    if batch:
+        check_hip(hip.uaii_hip_attention_batch(ptr(both), ld, I64(n), ptr(kc), ptr(vc), KV_F16, I64(seq), ptr(lens), None, None, I64(0), I64(0),
+                                               heads, kv, hd, None, ptr(out), ld, None))
+    else:
+        check_hip(hip.uaii_hip_attention_prompt(ptr(both), ld, I64(n), ptr(kc), ptr(vc), KV_F16, I64(seq), I64(6), I64(0), None, heads, kv, hd,
+                                                None, ptr(out), ld, None))
+    got, at, none = both.cpu().numpy(), np.arange(seq), np.zeros(1)
+    assert np.array_equal(got[:, :width], q) and (got[:, 2 * width :] == -7.0).all()
+    for s in range(n):
+        for h in range(heads):
+            c, hi = (s, int(lens[s])) if batch else (0, 7 + s)
+            w, tol = attend(q[s : s + 1, h * hd : (h + 1) * hd], kx[c, h // 2], vx[c, h // 2], at, none, none, np.array([hi]), 0.125, 0.0, 0.0)
+            close(got[s : s + 1, width + h * hd : width + (h + 1) * hd], w, tol)
+
+
 # ---- attention of prompt rows ----------------------------------------------------------------
 
 
@@ -463,6 +515,20 @@ def test_prompt_long(hip, t, shape):
     """Blocks of every kind of a longer prompt; some rows are checked."""
     check_prompt(hip, np.random.default_rng(17), t, *shape, m=1100, p0=500, window=700, which=[0, 1, 199, 200, 201, 555, 1023, 1024, 1099])
     check_prompt(hip, np.random.default_rng(18), t, *shape, m=40, p0=6000, which=[0, 7, 39])
+
+
+def test_prompt_scale_not_finite(hip):
+    """An 8-bit row with a scale of infinity reaches the queries that see it and no others."""
+    rng = np.random.default_rng(19)
+    heads, kv, hd, m = 4, 2, 64, 100
+    (kc, _), (vc, _) = (pack(rows(rng, 1, kv, m, hd), KV_Q8) for _ in range(2))
+    scales = vc[0, kv * m * hd : kv * m * (hd + 4)].view(torch.float32)
+    scales[50] = math.inf
+    dq, out = torch.from_numpy(rows(rng, m, heads * hd)).cuda(), torch.zeros(m, heads, hd, device="cuda")
+    check_hip(hip.uaii_hip_attention_prompt(ptr(dq), I64(heads * hd), I64(m), ptr(kc), ptr(vc), KV_Q8, I64(m), I64(0), I64(0), None, heads, kv,
+                                            hd, None, ptr(out), I64(heads * hd), None))
+    got = out.cpu().numpy()
+    assert np.isfinite(got[:50]).all() and np.isfinite(got[:, 2:]).all() and not np.isfinite(got[50:, :2]).any()
 
 
 # ---- the largest offsets, streams, graphs, and all of it together --------------------------------

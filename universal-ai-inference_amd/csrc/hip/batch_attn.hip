@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(256, HD == 256 && (TYPE == KV_F32 || !PACK) ? 
     }
     __syncthreads();
     const float unit = TYPE == KV_F32 ? 1.0f : pow2i(-row_exponent(qtop[crow])) * (SC ? kQ8Unit : 1.0f);
-    const float to_cap = capped ? unit / a.cap : 0.0f;
+    const float to_cap = capped ? fminf(unit / a.cap, 0x1p127f) : 0.0f;  // finite: a score of 0 stays 0
     const float mul = (capped ? a.cap : unit) * kLog2e;  // scores in base 2
     const float slope = sloped && crow < rows ? a.slopes[head0 + crow] * kLog2e : 0.0f;
 
@@ -669,7 +669,7 @@ int resident_blocks(int type, int hd, bool pack) {
 
 struct Plan {
   int G, groups, rc, blocks, parts, splits, fold;
-  bool pack;
+  bool pack, too_many;  // too_many: units, for 32-bit numbers
   RowsAttnArgs rows;
   size_t part, slots, whole, info;  // bytes of the scratch's parts
   size_t bytes() const { return part + slots + whole + info; }
@@ -707,6 +707,7 @@ Plan plan_of(const SeqAttnArgs& a) {
     const int64_t held = (a.window ? std::min<int64_t>(a.window, a.max_seq + p.fold) : a.max_seq + p.fold) + (p.fold ? 31 : 0);
     const int64_t parts = (held + UNIT - 1) / UNIT, resident = resident_blocks(a.type, a.hd, p.pack);
     p.parts = heads * parts <= 2 * resident ? (int)parts : 0;
+    p.too_many = heads * parts > INT32_MAX;
     p.blocks = (int)std::min<int64_t>(heads * parts, p.parts ? 2 * resident : resident);
     p.slots = pad256((p.parts ? 1 : 2) * (size_t)p.blocks * p.rc * row);
     p.info = p.parts ? 0 : pad256((size_t)heads * sizeof(int2));
@@ -727,7 +728,7 @@ size_t seq_attn_scratch(const SeqAttnArgs& a) { return plan_of(a).bytes(); }
 
 hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
   Plan p = plan_of(a);
-  if (a.rows <= 0 || (p.bytes() > 0 && !scratch)) return hipErrorInvalidValue;
+  if (a.rows <= 0 || p.too_many || (p.bytes() > 0 && !scratch)) return hipErrorInvalidValue;
   JoinArgs j{};
   j.a = a;
   j.G = p.G;

@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
     if constexpr (QL) __syncthreads();
   }
   const bool capped = a.cap > 0.0f, sloped = a.slopes != nullptr;
-  const float to_cap = capped ? unit / a.cap : 0.0f;
+  const float to_cap = capped ? fminf(unit / a.cap, 0x1p127f) : 0.0f;  // finite: a score of 0 stays 0
   const float mul = (capped ? a.cap : unit) * kLog2e;  // scores in base 2
   const float slope = sloped ? a.slopes[head] * kLog2e : 0.0f;
 
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
     if constexpr (TYPE == KV_Q8) {
       constexpr int VWAVE = TK == 64 ? 1 : 0;  // the wave that holds the values' factors
       if (rw == VWAVE) {
-        const bool factor = tid >= TK, out = factor && screg != screg;
+        const bool factor = tid >= TK, out = factor && !(fabsf(screg) < INFINITY);
         const bool any = __any(out);
         if (factor) to.at[tid - TK][0] = out;
         screg = out ? 0.0f : screg;

@@ -15,6 +15,7 @@ namespace {
 
 constexpr int kErrArg = -1;  // invalid argument
 constexpr int64_t kMaxPositions = (int64_t)1 << 30;  // positions and steps past them are 32-bit in the kernels
+constexpr float kMaxCap = 1e20f;  // scores over a larger one could pass the lower end of f32
 
 hipStream_t S(void* s) { return static_cast<hipStream_t>(s); }
 
@@ -26,11 +27,14 @@ bool layout_ok(int kv_type, int n_kv_heads, int head_dim, int64_t max_seq) {
 bool aligned16(const void* p) { return p && (uintptr_t)p % 16 == 0; }
 bool aligned4(const void* p) { return p && (uintptr_t)p % 4 == 0; }
 
-// [rows][ld] floats of which `width` a row are used
+// [rows][ld] floats of which `width` a row are used. Rows of one pitch may lie between each
+// other, as the columns of one wide buffer do.
 bool overlap(const float* a, int64_t lda, const float* b, int64_t ldb, int64_t rows, int64_t width) {
   const uintptr_t a0 = (uintptr_t)a, a1 = a0 + (uintptr_t)((rows - 1) * lda + width) * 4;
   const uintptr_t b0 = (uintptr_t)b, b1 = b0 + (uintptr_t)((rows - 1) * ldb + width) * 4;
-  return a0 < b1 && b0 < a1;
+  if (a1 <= b0 || b1 <= a0) return false;
+  const uintptr_t pitch = (uintptr_t)lda * 4, used = (uintptr_t)width * 4, from = (a0 > b0 ? a0 - b0 : b0 - a0) % pitch;
+  return lda != ldb || from < used || pitch - from < used;
 }
 
 // The rows of uaii_hip_kv_append_batch and uaii_hip_kv_read.
@@ -84,7 +88,7 @@ bool attn_args(const float* q, int64_t ldq, int64_t rows, const void* kcache, co
   a->max_seq = max_seq;
   a->seq_bytes = kv_seq_bytes(kv_type, n_kv_heads, max_seq, head_dim);
   if (o) {
-    if (o->struct_size < sizeof(*o) || !std::isfinite(o->scale) || !std::isfinite(o->softcap) || o->softcap < 0.0f ||
+    if (o->struct_size < sizeof(*o) || !std::isfinite(o->scale) || !(o->softcap >= 0.0f && o->softcap <= kMaxCap) ||
         o->window < 0 || (o->slopes && !aligned4(o->slopes)))
       return false;
     a->scale = o->scale;
