@@ -95,11 +95,21 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
   const int kvh = (int)(blockIdx.x % (unsigned)a.n_kv);
   const int sx = (int)(blockIdx.x / (unsigned)a.n_kv);
   const int split = sx % r.splits;
-  const int nx = (int)((r.R + MR * NR - 1) / (MR * NR));
-  const int64_t row_at = (int64_t)(nx - 1 - sx / r.splits) * (MR * NR) + MR * rw + col;  // the longest first
-  const bool valid = row_at < r.R;
-  const int64_t row = valid ? row_at : r.R - 1;
-  const int query = (int)(row / r.G), head = kvh * r.G + (int)(row % r.G);
+  const uint32_t R = (uint32_t)r.R, nx = (R + MR * NR - 1) / (MR * NR);
+  const uint32_t row_at = (nx - 1 - (uint32_t)(sx / r.splits)) * (MR * NR) + MR * rw + col;  // the longest first
+  const bool valid = row_at < R;
+  const uint32_t row = valid ? row_at : R - 1;
+  const int query = (int)(row / (uint32_t)r.G), head = kvh * r.G + (int)(row - (uint32_t)query * r.G);
+
+  // q, before anything that the way to the first tile waits for
+  constexpr int LC = QL ? NC / NK : NC;  // chunks that the wave loads: all, or its share where LDS holds q
+  auto chunk = [&](int i) { return QL ? i * NK + kg : i; };
+  f4_t qv[LC][2];
+#pragma unroll
+  for (int i = 0; i < LC; ++i) {
+    const float* at = a.q + (int64_t)query * a.ldq + (int64_t)head * a.hd + min(CD * chunk(i) + 8 * h, a.hd - 8);
+    qv[i][0] = *reinterpret_cast<const f4u_t*>(at), qv[i][1] = *reinterpret_cast<const f4u_t*>(at + 4);
+  }
 
   // positions [lo, hi) of the keys that the row sees, and its own
   int pos, lo = 0, hi;
@@ -182,25 +192,16 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
   h8_t qhi[QL ? 1 : NC], qlo[QL ? 1 : NC];
   float unit;  // of a raw product
   {
-    const float* qp = a.q + (int64_t)query * a.ldq + (int64_t)head * a.hd;
-    constexpr int LC = QL ? NC / NK : NC;  // chunks that the wave loads: all, or its share where LDS holds q
-    auto chunk = [&](int i) { return QL ? i * NK + kg : i; };
-    float qv[LC][8], top = 0.0f;
-#pragma unroll
-    for (int i = 0; i < LC; ++i) {
-      const float* at = qp + min(CD * chunk(i) + 8 * h, a.hd - 8);
-      const f4_t x0 = *reinterpret_cast<const f4u_t*>(at), x1 = *reinterpret_cast<const f4u_t*>(at + 4);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) qv[i][k] = k < 4 ? x0[k] : x1[k - 4];
-    }
+    float top = 0.0f;
     // behind q, so that nothing waits for the tile with it
     if (mine < k1) load_tile(mine);
 #pragma unroll
     for (int i = 0; i < LC; ++i)
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        qv[i][k] = CD * chunk(i) + 8 * h < a.hd ? qv[i][k] * a.scale : 0.0f;
-        top = fmaxf(top, fabsf(qv[i][k]));
+        const float x = CD * chunk(i) + 8 * h < a.hd ? qv[i][k / 4][k % 4] * a.scale : 0.0f;
+        qv[i][k / 4][k % 4] = x;
+        top = fmaxf(top, fabsf(x));
       }
     top = row_max(top);
     if constexpr (QL) {
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
 #pragma unroll
       for (int k = 0; k < 8; k += 2) {
         h2_t x, y;
-        split2(qv[i][k] * up, qv[i][k + 1] * up, x, y);
+        split2(qv[i][k / 4][k % 4] * up, qv[i][k / 4][k % 4 + 1] * up, x, y);
         hi8[k] = x.x, hi8[k + 1] = x.y, lo8[k] = y.x, lo8[k + 1] = y.y;
       }
       if constexpr (QL) qs[64 * chunk(i) + lane] = hi8, qs[64 * (NC + chunk(i)) + lane] = lo8;
