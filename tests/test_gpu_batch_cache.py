@@ -200,6 +200,33 @@ def test_8_bit_rounding(hip):
     assert (np.abs(back[fine] - x[fine].astype(np.float64)) <= d[fine, None].astype(np.float64) * 0.5001).all()
 
 
+@pytest.mark.parametrize("hd", [16, 80, 256])
+def test_8_bit_rounding_of_many(hip, hd):
+    """Rows of all sizes, a third of them on halves of a step, a third a last place beside one."""
+    rng = np.random.default_rng(hd)
+    n = 600_000 // hd
+    x = rows(rng, n, hd)
+    half = (rng.integers(-253, 254, (n, hd)) * 0.5).astype(np.float32)
+    half[:, 0] = 127.0
+    x[n // 3 :] = half[n // 3 :]
+    beside = np.nextafter(half, np.where(rng.random((n, hd)) < 0.5, -np.inf, np.inf).astype(np.float32))
+    beside[:, 0] = 127.0
+    x[2 * n // 3 :] = beside[2 * n // 3 :]
+    with np.errstate(over="ignore", under="ignore"):
+        x *= (2.0 ** rng.uniform(-149, 121, (n, 1))).astype(np.float32)
+        x[::2] *= np.float32(1.0 / 3.0)
+    assert np.isfinite(x).all()
+    q, d = quantised(x)
+    caches = [torch.zeros(seq_bytes(KV_Q8, 1, n, hd), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    dx = torch.from_numpy(x).cuda()
+    check_hip(hip.uaii_hip_kv_append_batch(ptr(dx), ptr(dx), I64(hd), ptr(caches[0]), ptr(caches[1]), KV_Q8, I64(1), I64(n), 1, hd, I64(n),
+                                           I64(0), None, None))
+    for c in caches:
+        got = c.cpu().numpy()
+        assert np.array_equal(got[n * hd : n * (hd + 4)].view(np.float32), d)
+        assert np.array_equal(got[: n * hd].reshape(n, hd), q)
+
+
 # ---- attention of a batch --------------------------------------------------------------------
 
 
