@@ -699,10 +699,12 @@ hipError_t by_width(const RowsAttnArgs& r, hipStream_t s) {
 // on f16 caches of head_dim 128: a block's way to its first tile and from its last one 10 k; a
 // turn (32 keys) 3.5 k where each wave stages its own tiles, 2.8 k where two share one, 2.4 k
 // where four do (1.6 times the first two with rows of 256); 1.35 times that with two blocks
-// on a CU. A split writes its rows' sums and the
-// join reads them: 12 bytes a cycle and CU, and its own way. (4012 rows of 8 heads over a window of 1500, KV_Q8: two row
-// waves 73 us, four and two splits 88; 10400 rows of one head of 256 over 1300: four row waves
-// and three splits 42 us, two row waves 70.)
+// on a CU. A split writes its rows' sums and the join reads them, 12 bytes a cycle and CU,
+// and takes its 50 of the join's way. (4012 rows of 8 heads over a window of 1500, KV_Q8:
+// two row waves 73 us, four and two splits 88; 10400 rows of one head of 256 over 1300: four
+// row waves and three splits 41 us, two row waves 70; 24 rows of one such head over 30000:
+// 128 splits 17, 64 21; 1024 rows of 8 f32 heads of 128 over 1256: four row waves and eight
+// splits 46, two and two 60.)
 void rows_attn_shape(RowsAttnArgs* r) {
   const SeqAttnArgs& a = r->a;
   int64_t most = a.n_prefix, mean = most;  // keys of a row
@@ -725,7 +727,7 @@ void rows_attn_shape(RowsAttnArgs* r) {
       const double turns = std::max(1.0, (waits > 1 ? mean : most) / 32.0 / nk / splits);
       const double shared = full > device_cus() && all > device_cus() ? 1.35 : 1.0;
       double cost = (waits > 1 ? (double)all / full + 0.3 : 1.0) * (10e3 + turns * turn * shared);
-      if (splits > 1 || r->prefix) cost += splits * (row_bytes / 12 + 400) + 4e3;
+      if (splits > 1 || r->prefix) cost += splits * (row_bytes / 12 + 50) + 4e3;
       if (best == 0 || cost < best) best = cost, r->nr = nr, r->splits = (int)splits;
     }
   }
