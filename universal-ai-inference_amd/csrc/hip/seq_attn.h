@@ -80,11 +80,11 @@ __device__ inline float weight_of(float m, float l, float M) {
   return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
 }
 
-// ---- rows_attn.hip: many rows over one cache -------------------------------------------
+// ---- many rows over one cache (rows_block.h) -------------------------------------------
 
 // Rows of one kv head are its G query heads' rows of query 0, of query 1, and so on:
-// row r is query r / G, head r % G. The keys are positions of one cache (kc, vc of `a`,
-// or its prefix).
+// row r is query r / G, head r % G. The keys are positions of one cache: kc, vc of `a`, or
+// its prefix.
 struct RowsAttnArgs {
   SeqAttnArgs a;
   int64_t R;      // rows of a kv head
@@ -94,7 +94,12 @@ struct RowsAttnArgs {
   float* part;    // [splits][n_kv][R][part_stride]
 };
 
+// The fewest row waves there is a kernel for: LDS and registers do not hold f32 rows' pairs
+// for a lone wave.
+constexpr int rows_least(int type, int hd) { return type != KV_F32 || hd <= 64 ? 1 : hd <= 128 ? 2 : 4; }
+
 void rows_attn_shape(RowsAttnArgs* r);  // nr and splits from the rest
-hipError_t launch_rows_attn(const RowsAttnArgs& r, hipStream_t s);
+int64_t rows_attn_blocks(const RowsAttnArgs& r);
+hipError_t launch_rows_attn(const RowsAttnArgs& r, hipStream_t s);  // a prompt's
 
 }  // namespace uaii_hip
