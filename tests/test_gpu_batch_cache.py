@@ -335,6 +335,21 @@ def test_batch_shared_prefix_options(hip, t, shape, n, prefix, opt):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("heads,window", [(8, 20), (8, 100), (40, 45)])
+def test_batch_shared_prefix_window(hip, t, heads, window):
+    """The same for many sequences and a narrow window; more query heads than a block has rows."""
+    check_batch(hip, np.random.default_rng(31), t, heads, 4, 32, lens=[(7 * i) % 45 for i in range(300)], seq=45, prefix=500, window=window,
+                slopes=True)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("window", [60, 97, 128, 129, 161, 200])
+def test_batch_prefix_in_a_window(hip, t, window):
+    """Windows that begin anywhere in a prefix read with the sequences' own keys."""
+    check_batch(hip, np.random.default_rng(32), t, 4, 2, 64, lens=[0, 1, 31, 32, 33, 96, 160, 160], seq=160, prefix=75, window=window)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
 @pytest.mark.parametrize("prefix", [0, 200])
 @pytest.mark.parametrize("opt", [dict(cap=30.0), dict(cap=0.5), dict(slopes=True), dict(window=1), dict(window=50), dict(window=150),
                                  dict(window=1 << 40), dict(scale=0.3), dict(scale=-0.1),

@@ -194,17 +194,6 @@ struct Plan {
   size_t bytes() const { return part + slots + whole + info; }
 };
 
-// Whether each sequence reads the prefix with its own keys, where that is little: a launch and
-// its partials are saved, and the reads after the first come from caches. Measured, read with
-// each sequence against once for all (us): f16, 8 heads of 128, 4 sequences over 100 keys 9.9,
-// 16.9, 32 over 500 (62 MB, 128 k keys of heads) 21.5, 22.0, 8 over 6000 (187 MB) 24.9, 22.7,
-// 48 over 2000 47.6, 35.4; KV_Q8, 4 heads of 64, 8 over 6000 (192 k keys) 19.8, 19.7, 5 over
-// 30011 28.1, 22.6.
-bool folds(const SeqAttnArgs& a) {
-  const int64_t keys = a.rows * a.n_prefix;
-  return a.n_prefix > 0 && keys * a.n_kv <= 192 << 10 && keys * kv_seq_bytes(a.type, a.n_kv, 1, a.hd) * 2 <= (int64_t)64 << 20;
-}
-
 size_t pad256(size_t n) { return (n + 255) / 256 * 256; }
 
 Plan plan_of(const SeqAttnArgs& a) {
@@ -218,24 +207,36 @@ Plan plan_of(const SeqAttnArgs& a) {
     rows_attn_shape(&p.rows);
     p.splits = p.rows.splits > 1 ? p.rows.splits : 0;
   } else {
-    p.fold = folds(a) ? a.n_prefix : 0;
+    // Each sequence reads the prefix with its own keys where that is at most half a unit more,
+    // or every unit then still has a block of its own, all on the device at once; else one
+    // read serves all. (us, read by each and by all; f16, 8 heads of 128, 50 keys each: 4
+    // sequences, prefix of 60 8.5, 10.4, of 500 10.7, 12.0; 32, of 60 10.8, 13.6, of 120 19.2,
+    // 13.9, of 250 14.3, 14.1, of 500 16.1, 14.8; 100, of 60 17.9, 19.1, of 500 39.9, 33.3; 8
+    // with 100, of 6000 24.7, 17.6. KV_Q8, 4 heads of 64: 4, of 60 9.2, 10.6, of 500 10.7,
+    // 10.3; 32, of 250 12.4, 10.7.)
+    const bool narrow = a.type != KV_F32 && p.G <= 8;
+    auto units_of = [&](bool pack, int fold) {  // the most there can be, and what goes with them
+      p.pack = pack;
+      p.rc = rows_of(pack);
+      p.groups = (p.G + p.rc - 1) / p.rc;
+      const int64_t seen = a.window ? std::min<int64_t>(a.window, a.max_seq + fold) : a.max_seq + fold;
+      return a.rows * a.n_kv * p.groups * ((seen + (fold ? 31 : 0) + UNIT - 1) / UNIT);
+    };
+    int64_t resident = resident_blocks(a.type, a.hd, narrow, 0);
+    if (a.n_prefix <= UNIT / 2 || units_of(narrow, a.n_prefix) <= resident) p.fold = a.n_prefix;
     const bool shared = a.n_prefix > p.fold;
-    p.pack = a.type != KV_F32 && (p.G <= 8 || shared);
-    p.rc = rows_of(p.pack);
-    p.groups = (p.G + p.rc - 1) / p.rc;
+    const int64_t units = units_of(narrow || (shared && a.type != KV_F32), p.fold);  // the kernel with a prefix has packed rows only
     if (shared) {
       p.rows.prefix = true;
       rows_attn_shape(&p.rows);
       p.splits = p.rows.splits;
       p.row_blocks = rows_attn_blocks(p.rows);
+      resident = std::max<int64_t>(device_cus(), resident_blocks(a.type, a.hd, p.pack, p.rows.nr) - p.row_blocks);
     }
     const int64_t heads = a.rows * a.n_kv * p.groups;
-    const int64_t held = (a.window ? std::min<int64_t>(a.window, a.max_seq + p.fold) : a.max_seq + p.fold) + (p.fold ? 31 : 0);
-    const int64_t parts = (held + UNIT - 1) / UNIT;
-    const int64_t resident = std::max<int64_t>(device_cus(), resident_blocks(a.type, a.hd, p.pack, shared ? p.rows.nr : 0) - p.row_blocks);
-    p.parts = heads * parts <= 2 * resident ? (int)parts : 0;
-    p.too_many = heads * parts > INT32_MAX;
-    p.blocks = (int)std::min<int64_t>(heads * parts, p.parts ? 2 * resident : resident);
+    p.parts = units <= 2 * resident ? (int)(units / heads) : 0;
+    p.too_many = units > INT32_MAX;
+    p.blocks = (int)std::min<int64_t>(units, p.parts ? 2 * resident : resident);
     p.slots = pad256((p.parts ? 1 : 2) * (size_t)p.blocks * p.rc * row);
     p.info = p.parts ? 0 : pad256((size_t)heads * sizeof(int2));
     if (shared) p.whole = p.parts ? 0 : pad256((size_t)heads * p.rc * row);

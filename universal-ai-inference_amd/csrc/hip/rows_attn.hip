@@ -13,11 +13,10 @@ __global__ void __launch_bounds__(256, 2) k_rows_attn(RowsAttnArgs r) {
   rows_block<TYPE, HD, NR, false>(r, blockIdx.x, lds);
 }
 
-// Blocks on the device at a time, by their LDS.
-int64_t full_of(const RowsAttnArgs& r, int nr) {
+// Whether a CU holds one block, not two, by its LDS.
+bool one_held(const RowsAttnArgs& r, int nr) {
   const bool f32 = r.a.type == KV_F32;
-  const bool one = r.a.hd > 128 ? nr < 4 || f32 : r.a.hd > 64 ? nr == 1 || (f32 && nr == 2) : f32 && nr == 1;
-  return (int64_t)device_cus() * (one ? 1 : 2);
+  return r.a.hd > 128 ? nr < 4 || f32 : r.a.hd > 64 ? nr == 1 || (f32 && nr == 2) : f32 && nr == 1;
 }
 
 int64_t row_blocks(const RowsAttnArgs& r, int nr) {
@@ -64,6 +63,11 @@ hipError_t by_width(const RowsAttnArgs& r, hipStream_t s) {
 // row waves and three splits 41 us, two row waves 70; 24 rows of one such head over 30000:
 // 128 splits 17, 64 21; 1024 rows of 8 f32 heads of 128 over 1256: four row waves and eight
 // splits 46, two and two 60.)
+//
+// Over a prefix there is one block a CU, and only one that leaves another the room for a
+// block of the sequences' own keys: where the lone waves of 8 f16 rows of 128 took all of
+// a CU, 20 sequences with a prefix of 2500 waited 29 us, now 24; two blocks of rows a CU
+// kept 48 sequences waiting 43 us, one 30.
 void rows_attn_shape(RowsAttnArgs* r) {
   const SeqAttnArgs& a = r->a;
   int64_t most = a.n_prefix, mean = most;  // keys of a row
@@ -77,7 +81,9 @@ void rows_attn_shape(RowsAttnArgs* r) {
   double best = 0;
   for (int nr = 4; nr >= least; nr /= 2) {
     const int nk = 4 / nr;
-    const int64_t blocks = row_blocks(*r, nr), full = r->prefix ? device_cus() : full_of(*r, nr);
+    const bool one = one_held(*r, nr);
+    if (r->prefix && one && nr < 4) break;
+    const int64_t blocks = row_blocks(*r, nr), full = (int64_t)device_cus() * (one || r->prefix ? 1 : 2);
     const double turn = (nr == 4 ? 2400 : nr == 2 ? 2800 : 3500) * (a.hd > 128 && nr < 4 ? 1.6 : a.hd > 64 ? 1.0 : 0.65) * (a.type == KV_F32 ? 1.5 : 1.0);
     for (int64_t splits : {(int64_t)1, full / 2 / blocks, full / blocks}) {
       splits = std::min<int64_t>({splits, 128, (most + 127) / 128});
