@@ -65,9 +65,9 @@ hipError_t by_width(const RowsAttnArgs& r, hipStream_t s) {
 // splits 46, two and two 60.)
 //
 // Over a prefix there is one block a CU, and only one that leaves another the room for a
-// block of the sequences' own keys: where the lone waves of 8 f16 rows of 128 took all of
-// a CU, 20 sequences with a prefix of 2500 waited 29 us, now 24; two blocks of rows a CU
-// kept 48 sequences waiting 43 us, one 30.
+// block of the sequences' own keys: with blocks of one row wave, which take all of a CU
+// (f16, 32/8 heads of 128), 20 sequences and a prefix of 2500 took 29 us, with others 24;
+// with two blocks of rows a CU 48 sequences and a prefix of 6000 took 43 us, with one 30.
 void rows_attn_shape(RowsAttnArgs* r) {
   const SeqAttnArgs& a = r->a;
   int64_t most = a.n_prefix, mean = most;  // keys of a row

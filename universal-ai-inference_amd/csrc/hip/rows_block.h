@@ -1,6 +1,30 @@
 // rows_block.h — what a block does in attention of many rows over one cache on the matrix
 // cores: the rows of a prompt (rows_attn.hip), or the queries of a batch over the prefix that
 // its sequences share (batch_attn.hip).
+//
+// One pass over the keys with the running maximum and sum of the softmax. A wave has 32 rows
+// (16 with rows of 256) and takes 32 keys a turn: S^T = K . Q^T puts a row's scores into the
+// lanes that hold its sums, so that maximum, sum and probabilities stay in registers, and the
+// probabilities are the operand of O^T += V^T . P^T as they lie; V is read from LDS
+// transposed. The next tile's loads stand between the matrix ops of the scores, its way into
+// LDS between those of the sums.
+//
+// Precision: a cache's values enter the f16 matrix ops as they are (f16), as whole numbers
+// 2^-9 (KV_Q8, a key's factor on its score, a value's on its probability) or as f16 pairs
+// hi + lo (f32, scaled by a power of two for each row); q and the probabilities are pairs.
+// So a product takes two matrix ops (f32: three) where plain f16 would take one, and results
+// stand within 2e-7 to 7e-7 of 64-bit ones, like f32 sums. Scores and probabilities are in
+// base 2; the maximum follows in steps of 2^4, 2^10 keeps small probabilities above f16's
+// subnormals, and D, a power of two over the values' factors so far, keeps p times factor
+// below f16's end.
+//
+// What bounds it: matrix ops and vector ops share a SIMD's two waves. f16 rows of 128 (4096
+// rows of 32/8 heads in three documents, 168 us): 413 TFLOP/s of the formula, 826 of matrix
+// ops where a large f16 library product reaches 1178; the matrix cores are busy 38 % of all
+// SIMD cycles, the vector units 34 %, and the rest is the longest blocks' end, where CUs have
+// run out of others, and each block's way to its first tile (5 us, of which a block beside it
+// hides a part). KV_Q8 with softcap and window (1003 rows over 1500 keys, 75 us): 29 vector
+// ops a score (7 for tanh, 6.5 for the bytes' way to f16), busy 64 %.
 #pragma once
 
 #include "seq_attn.h"
