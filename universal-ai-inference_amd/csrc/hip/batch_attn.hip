@@ -281,7 +281,6 @@ hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
     b.slots = reinterpret_cast<float*>(scratch + p.part);
     b.whole = reinterpret_cast<float*>(scratch + p.part + p.slots);
     b.info = reinterpret_cast<int2*>(scratch + p.part + p.slots + p.whole);
-    b.pre = j.part;
     b.pre_splits = p.splits;
     b.blocks = p.blocks;
     b.parts = p.parts;

@@ -25,7 +25,6 @@ struct BatchArgs {
   float* slots;        // [2 blocks][RC][part_stride]: a block's first and last run
   float* whole;        // [n_seq * n_kv * groups][RC][part_stride], with a prefix only
   int2* info;          // for each (sequence, kv head, group): its first block, and how many follow
-  const float* pre;    // partials over the prefix (RowsAttnArgs::part)
   int pre_splits, blocks;
   int fold;            // keys of a prefix that each sequence reads with its own
   int parts;           // > 0: a block for each of so many units of every head, used or not

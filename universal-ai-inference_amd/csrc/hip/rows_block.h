@@ -24,7 +24,7 @@
 // SIMD cycles, the vector units 34 %, and the rest is the longest blocks' end, where CUs have
 // run out of others, and each block's way to its first tile (5 us, of which a block beside it
 // hides a part). KV_Q8 with softcap and window (1003 rows over 1500 keys, 75 us): 29 vector
-// ops a score (7 for tanh, 6.5 for the bytes' way to f16), busy 64 %.
+// ops a score (7 for tanh, 6.5 for the bytes' way to f16), busy 51 %, the matrix cores 26 %.
 #pragma once
 
 #include "seq_attn.h"
