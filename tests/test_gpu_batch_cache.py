@@ -1,10 +1,11 @@
 """Caches of a batch: rows written and read back, and attention over them.
 
 Every result is held against the operator's definition in 64 bits. Tolerances of the
-attentions are worked out for each output value from the inputs (see `bound`); what the
+attentions are worked out for each output value from the inputs (see `attend`); what the
 caches hold is compared exactly."""
 import ctypes
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -619,22 +620,20 @@ def test_streams(hip):
     """Calls on six streams and the null stream at once give the bits of the same calls alone."""
     made = [run_batch(hip, np.random.default_rng(20 + i), [KV_Q8, KV_F16][i % 2], 8, 2, 64, lens=[700 + i, 3, 50], seq=800, prefix=64 * i)
             for i in range(7)]
-    want = []
+    want, outs = [], []
     for call, _, _ in made:
         out, _ = call(None)
         torch.cuda.synchronize()
         want.append(out.clone())
-        out.fill_(-7.0)
+        outs.append(out.fill_(-7.0))
     streams = [torch.cuda.Stream() for _ in range(6)]
     torch.cuda.synchronize()
     for _ in range(4):
         for i, (call, _, _) in enumerate(made):
             call(ctypes.c_void_p(streams[i].cuda_stream) if i < 6 else None)
     torch.cuda.synchronize()
-    for i, (call, _, _) in enumerate(made):
-        out, _ = call(None)
-        torch.cuda.synchronize()
-        assert torch.equal(out, want[i])
+    for out, w in zip(outs, want):
+        assert torch.equal(out, w)
 
 
 def test_serving_run(hip):
@@ -711,3 +710,83 @@ def test_serving_run(hip):
             state["past"] += 1
             state["lens"] += 1
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+def test_graph_of_large_calls(hip, t):
+    """Units in shares, a shared prefix and split prompt rows in one graph, replayed with other lengths
+    and queries between eager calls: the same bits as those."""
+    rng = np.random.default_rng(40)
+    heads, kv, hd, n, seq, prefix, m = 8, 4, 64, 70, 1100, 900, 30
+    width = heads * hd
+    new = lambda *shape: torch.randn(*shape, device="cuda", generator=gen)  # noqa: E731
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    size, psize = seq_bytes(t, kv, seq, hd), seq_bytes(t, kv, prefix, hd)
+    kc, vc = (torch.zeros(n * size, dtype=torch.uint8, device="cuda") for _ in range(2))
+    kp, vp = (torch.zeros(psize, dtype=torch.uint8, device="cuda") for _ in range(2))
+    for k, v, s, count, to in ((kc, vc, seq, n, seq), (kp, vp, prefix, 1, prefix)):
+        a, b = new(count * to, kv * hd), new(count * to, kv * hd)
+        check_hip(hip.uaii_hip_kv_append_batch(ptr(a), ptr(b), I64(kv * hd), ptr(k), ptr(v), t, I64(count), I64(to), kv, hd, I64(s), I64(0),
+                                               None, None))
+        torch.cuda.synchronize()
+    q, lens = new(n, width), torch.zeros(n, dtype=torch.int32, device="cuda")
+    outs = [[torch.zeros(n, width, device="cuda"), torch.zeros(n, width, device="cuda"), torch.zeros(m, width, device="cuda")] for _ in range(2)]
+
+    def calls(to, stream):
+        for out, pre in ((to[0], 0), (to[1], prefix)):
+            check_hip(hip.uaii_hip_attention_batch(ptr(q), I64(width), I64(n), ptr(kc), ptr(vc), t, I64(seq), ptr(lens), ptr(kp), ptr(vp),
+                                                   I64(prefix), I64(pre), heads, kv, hd, None, ptr(out), I64(width), stream))
+        check_hip(hip.uaii_hip_attention_prompt(ptr(q), I64(width), I64(m), ptr(kc), ptr(vc), t, I64(seq), I64(seq - m), I64(0), None, heads, kv,
+                                                hd, None, ptr(to[2]), I64(width), stream))
+
+    calls(outs[0], None)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        calls(outs[1], ctypes.c_void_p(torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    for i in range(4):
+        lens.copy_(torch.from_numpy(rng.integers(0, [5, seq, 1, seq][i] + 1, n).astype(np.int32)))
+        q.copy_(new(n, width))
+        for o in outs[0] + outs[1]:
+            o.fill_(-7.0)
+        torch.cuda.synchronize()
+        calls(outs[0], None)
+        graph.replay()
+        calls(outs[0], None)
+        torch.cuda.synchronize()
+        for a, b in zip(*outs):
+            assert torch.equal(a, b) and torch.isfinite(a).all()
+    assert float(outs[0][1].abs().max()) > 0
+
+
+def test_threads(hip):
+    """Calls from four threads, each on a stream of its own, give the bits of the same calls alone."""
+    made = [run_batch(hip, np.random.default_rng(50 + i), TYPES[i % 3], 8, 2, 64, lens=[(97 * j) % 400 for j in range(30)], seq=400, prefix=[0, 700][i % 2])
+            for i in range(4)]
+    want, outs = [], []
+    for call, _, _ in made:
+        out, _ = call(None)
+        torch.cuda.synchronize()
+        want.append(out.clone())
+        outs.append(out.fill_(-7.0))
+    streams = [torch.cuda.Stream() for _ in made]
+    torch.cuda.synchronize()
+    failed = []
+
+    def work(i):
+        try:
+            for _ in range(20):
+                made[i][0](ctypes.c_void_p(streams[i].cuda_stream))
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(made))]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for out, w in zip(outs, want):
+        assert torch.equal(out, w)
