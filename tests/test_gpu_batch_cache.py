@@ -335,6 +335,16 @@ def test_batch_shared_prefix_options(hip, t, shape, n, prefix, opt):
     check_batch(hip, np.random.default_rng(5), t, *shape, lens=[(7 * i) % 45 for i in range(n)], seq=45, prefix=prefix, **opt)
 
 
+@pytest.mark.parametrize("t,shape,n,prefix", [
+    (KV_F32, (16, 4, 64), 165, 128), (KV_F32, (64, 8, 64), 139, 287), (KV_F32, (32, 4, 128), 163, 128), (KV_F32, (8, 8, 256), 95, 128),
+    (KV_F16, (8, 8, 64), 119, 128), (KV_Q8, (8, 8, 64), 119, 128), (KV_F16, (64, 8, 64), 133, 160), (KV_Q8, (4, 4, 64), 150, 133),
+    (KV_F16, (64, 8, 64), 154, 302), (KV_Q8, (64, 8, 64), 154, 302), (KV_F16, (4, 4, 128), 142, 128), (KV_F16, (64, 8, 128), 144, 360),
+    (KV_Q8, (64, 8, 128), 144, 360), (KV_F16, (8, 8, 256), 78, 128), (KV_Q8, (8, 8, 256), 78, 128)], ids=str)
+def test_batch_shared_prefix_of_many(hip, t, shape, n, prefix):
+    """One, two and four row waves, with and without splits."""
+    check_batch(hip, np.random.default_rng(33), t, *shape, lens=[(7 * i) % 20 for i in range(n)], seq=45, prefix=prefix)
+
+
 @pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
 @pytest.mark.parametrize("heads,window", [(8, 20), (8, 100), (40, 45)])
 def test_batch_shared_prefix_window(hip, t, heads, window):
@@ -558,6 +568,32 @@ def test_prompt_long(hip, t, shape):
     """Blocks of every kind of a longer prompt; some rows are checked."""
     check_prompt(hip, np.random.default_rng(17), t, *shape, m=1100, p0=500, window=700, which=[0, 1, 199, 200, 201, 555, 1023, 1024, 1099])
     check_prompt(hip, np.random.default_rng(18), t, *shape, m=40, p0=6000, which=[0, 7, 39])
+
+
+# (shape, rows, position of the first): one, two and four row waves, with and without splits
+KINDS = [((32, 8, 64), 346, 325), ((8, 4, 64), 1351, 20), ((1, 1, 128), 1, 281), ((16, 4, 128), 680, 777), ((8, 8, 128), 1500, 0),
+         ((32, 8, 128), 1700, 3), ((1, 1, 256), 1, 264), ((4, 2, 256), 359, 110), ((4, 4, 256), 387, 144), ((16, 8, 256), 900, 0)]
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape,m,p0", KINDS, ids=str)
+def test_prompt_kinds(hip, t, shape, m, p0):
+    which = sorted({0, m // 3, m // 2, max(m - 40, 0), m - 1} | set(range(31, m, 97)))
+    check_prompt(hip, np.random.default_rng(34), t, *shape, m=m, p0=p0, which=which)
+    check_prompt(hip, np.random.default_rng(35), t, *shape, m=m, p0=p0, which=which[::2], cap=8.0, slopes=True, window=max(m // 2, 3),
+                 bidir=p0 + m // 4, first=[max(0, p0 + i - 300 + 150 * (i % 3)) for i in range(m)], spread=3.0)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape,m", [((8, 8, 128), 1500), ((32, 8, 64), 700), ((16, 8, 256), 900)], ids=str)
+def test_prompt_documents_of_many(hip, t, shape, m):
+    """Documents whose values are not finite, next to others, in blocks of four row waves."""
+    ends = [0, m // 5, m // 5 + 130, m // 2, m // 2 + 1, m]
+    first = np.concatenate([np.full(b - a, a) for a, b in zip(ends, ends[1:])])
+    bad = slice(ends[1], ends[2])
+    first[bad] = 1 << 30
+    which = [i for i in range(0, m, 53)] + [ends[1] - 1, ends[1], ends[2] - 1, ends[2], ends[3] - 1, ends[3], ends[4], m - 1]
+    check_prompt(hip, np.random.default_rng(36), t, *shape, m=m, p0=0, first=first.tolist(), poison=bad, which=sorted(set(which)))
 
 
 def test_prompt_scale_not_finite(hip):
