@@ -379,6 +379,14 @@ def test_batch_of_many(hip, t, n):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("heads,window,prefix", [(8, 0, 0), (8, 60, 0), (40, 0, 0), (8, 0, 40)])
+def test_batch_of_many_short(hip, t, heads, window, prefix):
+    """At most 128 keys for each of many sequences, and sequences with none."""
+    check_batch(hip, np.random.default_rng(37), t, heads, 8, 64, lens=[(i * 31) % 61 * (i % 5 != 2) for i in range(300)],
+                seq=300 if window else 60, window=window, prefix=prefix)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
 def test_batch_peaked(hip, t):
     """Scores that one key rules, found late, and keys of unlike size."""
     check_batch(hip, np.random.default_rng(7), t, 8, 2, 64, lens=[900, 333], seq=900, prefix=400, spread=20.0)

@@ -123,7 +123,14 @@ __device__ __forceinline__ void batch_block(const BatchArgs& b, unsigned block, 
     const int hx = (int)block / b.parts, uu = (int)block % b.parts;
     s = hx / H;
     const int n = span_of(a, b.fold, s).units();
-    if (uu >= n) return;
+    if (uu >= n) {
+      if (b.parts == 1 && b.pre_splits == 0) {  // no join follows: a sequence with no keys
+        const int kvh = hx % H / b.groups, r0 = hx % b.groups * RC, rows = min(RC, b.G - r0);
+        float* out = a.out + (int64_t)s * a.ldo + (int64_t)(kvh * b.G + r0) * a.hd;
+        for (int x = tid; x < rows * a.hd; x += 256) out[x] = 0.0f;
+      }
+      return;
+    }
     base = 0;
     u = hx % H * n + uu;
     u1 = u + 1;
@@ -273,8 +280,10 @@ __device__ __forceinline__ void batch_block(const BatchArgs& b, unsigned block, 
         qv[e] = qr < rows && qd < a.hd ? qv[e] * a.scale : 0.0f;
         top = fmaxf(top, fabsf(qv[e]));
       }
-#pragma unroll
-      for (int k = 8; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor(top, k, 64));
+      top = fmaxf(top, dpp_mov<0xB1>(top));   // quad_perm [1,0,3,2]
+      top = fmaxf(top, dpp_mov<0x4E>(top));   // quad_perm [2,3,0,1]
+      top = fmaxf(top, dpp_mov<0x141>(top));  // row_half_mirror
+      top = fmaxf(top, dpp_mov<0x140>(top));  // row_mirror
       if ((tid & 15) == 0) qtop[qr] = top;
       const float up = TYPE == KV_F32 ? 1.0f : pow2i(row_exponent(top));
       if (qr < RC) {

@@ -296,8 +296,11 @@ __device__ __forceinline__ void rows_block(const RowsAttnArgs& r, unsigned block
         const float mag = fabsf(v[k]);
         top = fmaxf(top, mag <= 3.4028235e38f ? mag : 0.0f);
       }
-#pragma unroll
-      for (int s = 1; s < PR; s <<= 1) top = fmaxf(top, __shfl_xor(top, s, 64));
+      top = fmaxf(top, dpp_mov<0xB1>(top));   // quad_perm [1,0,3,2]
+      top = fmaxf(top, dpp_mov<0x4E>(top));   // quad_perm [2,3,0,1]
+      top = fmaxf(top, dpp_mov<0x141>(top));  // row_half_mirror
+      if constexpr (PR >= 16) top = fmaxf(top, dpp_mov<0x140>(top));  // row_mirror
+      if constexpr (PR >= 32) top = fmaxf(top, __shfl_xor(top, 16, 64));
       const int e = row_exponent(top);
       const float up = pow2i(e);
       h8_t hi8, lo8;
