@@ -19,11 +19,11 @@
 // below f16's end.
 //
 // What bounds it: matrix ops and vector ops share a SIMD's two waves. f16 rows of 128 (4096
-// rows of 32/8 heads in three documents, 168 us): 413 TFLOP/s of the formula, 826 of matrix
+// rows of 32/8 heads in three documents, 162 us): 427 TFLOP/s of the formula, 855 of matrix
 // ops where a large f16 library product reaches 1178; the matrix cores are busy 38 % of all
 // SIMD cycles, the vector units 34 %, and the rest is the longest blocks' end, where CUs have
 // run out of others, and each block's way to its first tile (5 us, of which a block beside it
-// hides a part). KV_Q8 with softcap and window (1003 rows over 1500 keys, 75 us): 29 vector
+// hides a part). KV_Q8 with softcap and window (1003 rows over 1500 keys, 73 us): 29 vector
 // ops a score (7 for tanh, 6.5 for the bytes' way to f16), busy 51 %, the matrix cores 26 %.
 #pragma once
 
