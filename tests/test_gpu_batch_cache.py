@@ -387,6 +387,25 @@ def test_batch_of_many_short(hip, t, heads, window, prefix):
 
 
 @pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape,n", [((8, 8, 64), 40), ((8, 4, 64), 90), ((8, 4, 128), 64), ((4, 4, 256), 65)], ids=str)
+@pytest.mark.parametrize("opt", [dict(), dict(prefix=300), dict(prefix=50, window=1300), dict(window=1200, cap=20.0, slopes=True)], ids=str)
+def test_batch_in_shares(hip, t, shape, n, opt):
+    """More units than blocks: heads cut anywhere, sequences with none between them."""
+    lens = [[0, 30, 1500, 129, 700, 1, 1501][i % 7] if i % 3 else 40 + i for i in range(n)]
+    check_batch(hip, np.random.default_rng(38), t, *shape, lens=lens, seq=1500, **opt)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("shape,n,seq", [((8, 2, 64), 3, 512), ((8, 8, 128), 17, 1024), ((8, 8, 128), 17, 1025), ((2, 1, 256), 5, 512), ((40, 4, 64), 33, 900)],
+                         ids=str)
+def test_batch_short_capacity(hip, t, shape, n, seq):
+    """A block a head up to a capacity, a block a unit behind it."""
+    lens = [[seq, 0, 1, 128, 129, 257, seq - 1, seq // 2][i % 8] for i in range(n)]
+    check_batch(hip, np.random.default_rng(39), t, *shape, lens=lens, seq=seq)
+    check_batch(hip, np.random.default_rng(39), t, *shape, lens=lens, seq=seq, prefix=33, window=seq - 40)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
 def test_batch_peaked(hip, t):
     """Scores that one key rules, found late, and keys of unlike size."""
     check_batch(hip, np.random.default_rng(7), t, 8, 2, 64, lens=[900, 333], seq=900, prefix=400, spread=20.0)

@@ -6,8 +6,8 @@
 // dealt out evenly to a grid that just fills the device: a block works through the runs of
 // units that fall to it, writes a finished head's rows to the output at once, and leaves
 // the partial results of its first and last run, where a head goes on in another block,
-// to the join. A batch of few units in all takes a block for each that its capacity allows,
-// and no block has to look for its share (7 sequences of up to 3000 KV_Q8 keys, 8/4 heads of
+// to the join. A short capacity takes a block for each head, and a batch of few units in all
+// one for each unit that its capacity allows: no block has to look for its share (7 sequences of up to 3000 KV_Q8 keys, 8/4 heads of
 // 192: 14 us, with shares of 64 keys 20; but with four blocks for each that the device holds,
 // 48 sequences of up to 400 keys and their prefix took 52 where shares took 45).
 //
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(64 * W) k_attn_join(JoinArgs j) {
     if (units > 0) {
       const int hx = kvh * j.groups + gr / j.rc;
       if (j.parts > 0) {
-        own = units;
+        own = j.parts == 1 ? 1 : units;
         at = j.slots + ((int64_t)row * H + hx) * j.parts * j.rc * stride;
         ahead = step = j.rc * stride;
       } else {
@@ -245,11 +245,16 @@ Plan plan_of(const SeqAttnArgs& a) {
     }
     const int64_t heads = a.rows * a.n_kv * p.groups;
     p.too_many = units > INT32_MAX;
-    // A unit at most for each head takes a block for each, however many, and no join (KV_Q8, 300
-    // windows of 100 keys, 8/8 heads of 256: 41 us, in shares and joined 44; f32, 150 of 128, 8/8
-    // of 64: 17 and 19).
-    p.parts = units <= 2 * resident || (units == heads && !p.too_many) ? (int)(units / heads) : 0;
-    p.blocks = (int)(p.parts ? units : std::min(units, resident));
+    // Short capacities take one block a head and no join: up to four units, or eight where the
+    // heads alone are blocks for half of the CUs and rows are not wide. (us, one block a head
+    // and a block a unit, all of the capacity used; KV_Q8, 8 heads of 64, one sequence: 256
+    // keys 6.3, 9.2, 512 keys 7.7, 9.3; with 40 keys in it 5.5, 7.6. f16, 8 heads of 128, one
+    // sequence of 768 11.2, 10.1; 16 sequences of 512 10.2, 13.4, of 1024 15.7, 22.9, of 2048
+    // 25.4, 27.0 (KV_Q8 16.7, 14.7); 12 windows of 1024, 8 heads of 256 39.8, 33.2.)
+    const int64_t most = a.hd <= 128 && heads >= device_cus() / 2 ? 8 : 4;
+    if (units <= most * heads && !p.too_many) p.parts = 1;
+    else if (units <= 2 * resident) p.parts = (int)(units / heads);
+    p.blocks = (int)(p.parts ? heads * p.parts : std::min(units, resident));
     if (p.parts != 1 || shared) p.slots = pad256((p.parts ? 1 : 2) * (size_t)p.blocks * p.rc * row);
     p.info = p.parts ? 0 : pad256((size_t)heads * sizeof(int2));
     if (shared) p.whole = p.parts ? 0 : pad256((size_t)heads * p.rc * row);
@@ -301,7 +306,7 @@ hipError_t launch_seq_attn(const SeqAttnArgs& a, char* scratch, hipStream_t s) {
         return hipGetLastError();
       });
     }
-    if (e != hipSuccess || (p.parts == 1 && p.splits == 0)) return e;  // each row has one part at most
+    if (e != hipSuccess || (p.parts == 1 && p.splits == 0)) return e;  // each row is written
     j.rc = p.rc;
     j.groups = p.groups;
     j.parts = p.parts;

@@ -27,7 +27,7 @@ struct BatchArgs {
   int2* info;          // for each (sequence, kv head, group): its first block, and how many follow
   int pre_splits, blocks;
   int fold;            // keys of a prefix that each sequence reads with its own
-  int parts;           // > 0: a block for each of so many units of every head, used or not
+  int parts;           // > 1: a block for each of so many units of every head, used or not; 1: one for all of a head's
 };
 
 __device__ inline f4_t mfma32(h8_t a, h8_t b, f4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -119,7 +119,7 @@ __device__ __forceinline__ void batch_block(const BatchArgs& b, unsigned block, 
   int s, base, u, u1;  // base: the first unit of sequence s
   int total = 0, blocks = 0;
   if (b.parts > 0) {
-    // few units in all: block by block, and those behind a head's last one have nothing to do
+    // block by block, and those behind a head's last unit have nothing to do
     const int hx = (int)block / b.parts, uu = (int)block % b.parts;
     s = hx / H;
     const int n = span_of(a, b.fold, s).units();
@@ -133,7 +133,7 @@ __device__ __forceinline__ void batch_block(const BatchArgs& b, unsigned block, 
     }
     base = 0;
     u = hx % H * n + uu;
-    u1 = u + 1;
+    u1 = u + (b.parts == 1 ? n : 1);
   } else {
     if (n_seq <= 64) {
       // a lane for each sequence, in every wave
