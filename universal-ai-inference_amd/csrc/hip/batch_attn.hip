@@ -217,13 +217,6 @@ Plan plan_of(const SeqAttnArgs& a) {
     rows_attn_shape(&p.rows);
     p.splits = p.rows.splits > 1 ? p.rows.splits : 0;
   } else {
-    // Each sequence reads the prefix with its own keys where that is at most half a unit more,
-    // or every unit then still has a block of its own, all on the device at once; else one
-    // read serves all. (us, read by each and by all; f16, 8 heads of 128, 50 keys each: 4
-    // sequences, prefix of 60 8.5, 10.4, of 500 10.7, 12.0; 32, of 60 10.8, 13.6, of 120 19.2,
-    // 13.9, of 250 14.3, 14.1, of 500 16.1, 14.8; 100, of 60 17.9, 19.1, of 500 39.9, 33.3; 8
-    // with 100, of 6000 24.7, 17.6. KV_Q8, 4 heads of 64: 4, of 60 9.2, 10.6, of 500 10.7,
-    // 10.3; 32, of 250 12.4, 10.7.)
     const bool narrow = a.type != KV_F32 && p.G <= 8;
     auto units_of = [&](bool pack, int fold) {  // the most there can be, and what goes with them
       p.pack = pack;
@@ -232,8 +225,26 @@ Plan plan_of(const SeqAttnArgs& a) {
       const int64_t seen = a.window ? std::min<int64_t>(a.window, a.max_seq + fold) : a.max_seq + fold;
       return a.rows * a.n_kv * p.groups * ((seen + (fold ? 31 : 0) + UNIT - 1) / UNIT);
     };
+    // Short capacities take one block a head and no join: up to four units, or eight where the
+    // heads alone are blocks for half of the CUs and rows are not wide. (us, one block a head
+    // and a block a unit, all of the capacity used; KV_Q8, 8 heads of 64, one sequence: 256
+    // keys 6.3, 9.2, 512 keys 7.7, 9.3; with 40 keys in it 5.5, 7.6. f16, 8 heads of 128, one
+    // sequence of 768 11.2, 10.1; 16 sequences of 512 10.2, 13.4, of 1024 15.7, 22.9, of 2048
+    // 25.4, 27.0 (KV_Q8 16.7, 14.7); 12 windows of 1024, 8 heads of 256 39.8, 33.2.)
+    auto one_block = [&](int64_t units) {
+      const int64_t heads = a.rows * a.n_kv * p.groups;
+      return units <= (a.hd <= 128 && heads >= device_cus() / 2 ? 8 : 4) * heads;
+    };
+    // Each sequence reads the prefix with its own keys where that is at most half a unit more;
+    // where one block a head still does, if the blocks do not read it too often; and where
+    // every unit still has a block of its own, all on the device at once. Else one read serves
+    // all. (us, read by each and by all, 50 keys each; f16, 8 heads of 128: 4 sequences, prefix
+    // of 60 6.1, 10.4, of 500 10.3, 12.0; 32, of 120 7.1, 13.1, of 500 10.3, 14.2; 100, of 60
+    // 13.4, 18.1, of 250 23.8, 24.1, of 500 31.4, 26.2; 8 with 100, of 6000 25.0, 17.6. KV_Q8, 4
+    // heads of 64: 4, of 500 11.0, 9.7; 32, of 250 8.0, 10.0; 8 with 200, of 1000 11.6, 11.5.)
     int64_t resident = resident_blocks(a.type, a.hd, narrow, 0);
-    if (a.n_prefix <= UNIT / 2 || units_of(narrow, a.n_prefix) <= resident) p.fold = a.n_prefix;
+    const int64_t folded = units_of(narrow, a.n_prefix);
+    if (a.n_prefix <= UNIT / 2 || (one_block(folded) && a.rows * a.n_kv * p.groups * a.n_prefix <= 192 << 10) || folded <= resident) p.fold = a.n_prefix;
     const bool shared = a.n_prefix > p.fold;
     const int64_t units = units_of(narrow || (shared && a.type != KV_F32), p.fold);  // the kernel with a prefix has packed rows only
     if (shared) {
@@ -245,14 +256,7 @@ Plan plan_of(const SeqAttnArgs& a) {
     }
     const int64_t heads = a.rows * a.n_kv * p.groups;
     p.too_many = units > INT32_MAX;
-    // Short capacities take one block a head and no join: up to four units, or eight where the
-    // heads alone are blocks for half of the CUs and rows are not wide. (us, one block a head
-    // and a block a unit, all of the capacity used; KV_Q8, 8 heads of 64, one sequence: 256
-    // keys 6.3, 9.2, 512 keys 7.7, 9.3; with 40 keys in it 5.5, 7.6. f16, 8 heads of 128, one
-    // sequence of 768 11.2, 10.1; 16 sequences of 512 10.2, 13.4, of 1024 15.7, 22.9, of 2048
-    // 25.4, 27.0 (KV_Q8 16.7, 14.7); 12 windows of 1024, 8 heads of 256 39.8, 33.2.)
-    const int64_t most = a.hd <= 128 && heads >= device_cus() / 2 ? 8 : 4;
-    if (units <= most * heads && !p.too_many) p.parts = 1;
+    if (one_block(units) && !p.too_many) p.parts = 1;
     else if (units <= 2 * resident) p.parts = (int)(units / heads);
     p.blocks = (int)(p.parts ? heads * p.parts : std::min(units, resident));
     if (p.parts != 1 || shared) p.slots = pad256((p.parts ? 1 : 2) * (size_t)p.blocks * p.rc * row);
