@@ -345,6 +345,16 @@ def test_batch_shared_prefix_of_many(hip, t, shape, n, prefix):
     check_batch(hip, np.random.default_rng(33), t, *shape, lens=[(7 * i) % 20 for i in range(n)], seq=45, prefix=prefix)
 
 
+@pytest.mark.parametrize("t,shape,n,prefix", [
+    (KV_F32, (64, 8, 64), 161, 157), (KV_F32, (8, 8, 64), 9, 2781), (KV_F32, (64, 8, 256), 181, 139), (KV_F32, (8, 8, 256), 146, 172),
+    (KV_F16, (16, 8, 64), 202, 128), (KV_Q8, (2, 2, 64), 162, 619), (KV_F16, (64, 8, 64), 190, 140), (KV_Q8, (8, 8, 64), 178, 151),
+    (KV_Q8, (32, 8, 128), 247, 128), (KV_F16, (1, 1, 128), 84, 2403), (KV_F16, (64, 8, 256), 155, 164), (KV_Q8, (8, 8, 256), 123, 204)], ids=str)
+def test_batch_prefix_read_once_for_many(hip, t, shape, n, prefix):
+    """The same, beyond what the sequences' own blocks would read of the prefix."""
+    assert n * shape[1] * prefix > 192 << 10
+    check_batch(hip, np.random.default_rng(41), t, *shape, lens=[(7 * i) % 12 for i in range(n)], seq=45, prefix=prefix)
+
+
 @pytest.mark.parametrize("t", TYPES, ids=NAMES.get)
 @pytest.mark.parametrize("heads,window", [(8, 20), (8, 100), (40, 45)])
 def test_batch_shared_prefix_window(hip, t, heads, window):
